@@ -184,6 +184,79 @@ int qi_qkv_norm_rope_i8(const int8_t* act_img, const float* act_img_scales, cons
                         const int8_t* w_txt, const float* w_txt_scales, const void* b_txt, const void* norms_bf16,
                         const float* pe, int nb, int n_img, int n_txt, void* qkv_f16, void* stream);
 
+/* ------------------------------------------------------------ prompt operators
+ * The two operators a causal text model needs to turn prompts into the text
+ * states qi_forward takes (the reference runs its text encoder on cuBLAS and a
+ * materialised softmax, cuda_kernels.cu:1162-1240): 16-bit floating point in
+ * and out, FP32 sums, no context, no device allocation, no state kept between
+ * calls.  Concurrent calls on any streams are independent, and both can be
+ * captured into a CUDA graph.  The current device must be the one that holds
+ * the buffers.                                                              */
+enum { QI_DT_BF16 = 0, QI_DT_F16 = 1, QI_DT_F32 = 2 };
+enum { QI_ACT_NONE = 0, QI_ACT_GELU = 1, QI_ACT_SILU = 2, QI_ACT_SWIGLU = 3 };
+
+/* Attention over packed sequences, with grouped heads:
+ *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h / G]) v[j, h / G],
+ *   G = heads / kv_heads.
+ * Sequence b has the query rows [q_begin[b], q_end[b]) of q and out and the
+ * key rows [k_begin[b], k_end[b]) of k and v (device arrays of `batch` int32;
+ * packed sequences pass an array of batch + 1 offsets as begin and the same
+ * array from its second entry as end; a cache with a slot per sequence passes
+ * each slot's start and fill).  The query ranges must not overlap.  With Lq
+ * queries and Lk keys, causal != 0 lets query i see the keys j <= i + Lk - Lq:
+ * the queries are the sequence's last Lq positions, so Lq = 1 is one new token
+ * against a cache.  A query that sees no key gives zeros.  Rows of out in no
+ * query range are not written.  What rows of k and v outside a sequence's
+ * range hold, or at positions a query does not see, does not reach that
+ * query's result, NaN and infinities included.
+ * Element (row, head, d) of x is x[row * x_row + head * x_head + d]; strides
+ * are in elements, positive and multiples of 8, pointers 16-byte aligned
+ * (QI_ERR_ALIGN); rows and heads of out must not overlap one another.  total_q and
+ * total_k are the rows of q / out and of k / v; ranges are clipped to them.
+ * dtype is QI_DT_BF16 or QI_DT_F16 (all four tensors).  head_dim is a multiple
+ * of 8, at most 128 (QI_ERR_UNSUPPORTED).  max_k >= the longest key range is a
+ * hint that decides how keys are split over the device: a wrong one costs
+ * time, not correctness.  workspace: at least
+ * qi_prompt_attention_workspace(...) bytes, 16-byte aligned, not used by any
+ * other call until this one has finished (QI_ERR_ARG when smaller; that size
+ * is 0 and workspace may be NULL when the keys are not split).
+ * Replaces attention_forward (cuda_kernels.cu:1162-1240) as the text encoder
+ * uses it; exact counterpart of qi_sage_attention for causal = 0.            */
+int qi_prompt_attention(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
+                        long long k_head, const void* v, long long v_row, long long v_head, void* out,
+                        long long o_row, long long o_head, int dtype, int heads, int kv_heads, int head_dim,
+                        const int* q_begin, const int* q_end, const int* k_begin, const int* k_end, int batch,
+                        int total_q, int total_k, int max_k, float scale, int causal, void* workspace,
+                        long long workspace_bytes, void* stream);
+/* Workspace bytes of qi_prompt_attention on the current device for these
+ * sizes, or a negative status.                                              */
+long long qi_prompt_attention_workspace(int heads, int kv_heads, int head_dim, int batch, int total_q, int total_k,
+                                        int max_k);
+
+/* Linear layer on 16-bit operands, the 16-bit counterpart of qi_linear_i8:
+ *   out[m, n] = residual[m, n] + gate[n] * act(sum_k x[m, k] w[n, k] + bias[n])
+ * x [M, K] and w [N, K] are dtype (QI_DT_BF16 or QI_DT_F16) with leading
+ * dimensions ldx and ldw, out [M, N] is out_dtype (dtype, or QI_DT_F32) with
+ * ldo, sums are FP32 and rounded once into out.  bias (dtype), gate (FP32) and
+ * residual (out_dtype, leading dimension ldr) may be NULL: 0, 1 and 0.
+ * act: QI_ACT_NONE, QI_ACT_GELU (tanh form), QI_ACT_SILU, or QI_ACT_SWIGLU,
+ * where w holds 2N rows and bias 2N values and
+ *   act(...) = silu(x . w[n] + bias[n]) * (x . w[N + n] + bias[N + n]).
+ * residual may be out itself (same pointer and leading dimension); otherwise
+ * out overlaps no input (QI_ERR_ARG).  Any M >= 0, N and K >= 1; all pointers
+ * 16-byte aligned and all leading dimensions multiples of 16 bytes
+ * (QI_ERR_ALIGN).
+ * Replaces the cuBLAS BF16 products with separate bias, activation and
+ * residual kernels behind them (cuda_kernels.cu:4535-4596).                 */
+int qi_linear_16bit(const void* x, long long ldx, int M, int K, const void* w, long long ldw, int N, int dtype,
+                    const void* bias, int act, const float* gate, const void* residual, long long ldr, void* out,
+                    long long ldo, int out_dtype, void* stream);
+
+/* Error report of the two prompt operators on the current device: waits for
+ * the device, then returns QI_ERR_DEVICE (and clears the word) if any call
+ * since the last check gave up a bounded wait, else QI_OK.                   */
+int qi_prompt_ops_check(void);
+
 /* ------------------------------------------------------------ model level */
 typedef struct qi_ctx qi_ctx;
 typedef struct qi_model qi_model;

@@ -237,6 +237,43 @@ int sage_quantize_fp8pv_launch(const void* q, const void* k, const void* v, int 
                                float* qs, int8_t* kc, float* ks, uint8_t* vt, int s_pad, float* vamax, float* vs,
                                cudaStream_t stream, const SideStream* side = nullptr);
 
+// ---------------------------------------------------------------- prompt operators
+// qi_prompt_attention's arguments, already checked (strides in elements).
+struct PromptAttnArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  long long q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;
+  int dtype, heads, kv_heads, head_dim;
+  const int* q_begin;
+  const int* q_end;
+  const int* k_begin;
+  const int* k_end;
+  int batch, total_q, total_k, max_k;
+  float scale;
+  int causal;
+  void* workspace;
+};
+long long prompt_attention_workspace(int heads, int kv_heads, int head_dim, int batch, int total_q, int max_k);
+int prompt_attention_launch(const PromptAttnArgs& a, cudaStream_t stream);
+// qi_linear_16bit's arguments, already checked.
+struct Linear16Args {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const float* gate;
+  const void* residual;
+  void* out;
+  long long ldx, ldw, ldr, ldo;
+  int M, N, K, dtype, out_dtype, act;
+};
+int linear16_launch(const Linear16Args& a, cudaStream_t stream);
+// Sets *bad and clears the operator's device error word if a bounded wait of
+// it gave up on the current device (the device is idle).
+int prompt_attention_take_error(int* bad);
+int linear16_take_error(int* bad);
+
 int cfg_euler_launch(float* x, const void* cond, const void* uncond, float cfg, float sigma, float sigma_next, int H,
                      int W, void* x_bf16, cudaStream_t stream);
 

@@ -53,6 +53,11 @@ B_NORMS = ["attn.norm_q.weight", "attn.norm_k.weight", "attn.norm_added_q.weight
 B_COUNT = 3 * len(L_NAMES) + 4
 
 EPI_STORE, EPI_GELU, EPI_RESIDUAL = 0, 1, 2
+# 16-bit operators: types and activations of the header.
+DT_BF16, DT_F16, DT_F32 = 0, 1, 2
+ACT_NONE, ACT_GELU, ACT_SILU, ACT_SWIGLU = 0, 1, 2, 3
+_DT16 = {torch.bfloat16: DT_BF16, torch.float16: DT_F16}
+_DT_OUT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float32: DT_F32}
 
 
 class QIError(RuntimeError):
@@ -109,6 +114,10 @@ def lib():
             "qi_ctx_set_fused_qkv_epilogue": ([vp, i], i),
             "qi_ctx_sync": ([vp, vp, i], i),
             "qi_exchange_plan": ([i, i, i, i, i, i, vp, vp, vp, vp], i),
+            "qi_prompt_attention": ([vp, ll, ll] * 4 + [i, i, i, i, vp, vp, vp, vp, i, i, i, i, f, i, vp, ll, vp], i),
+            "qi_prompt_attention_workspace": ([i] * 7, ll),
+            "qi_linear_16bit": ([vp, ll, i, i, vp, ll, i, i, vp, i, vp, vp, ll, vp, ll, i, vp], i),
+            "qi_prompt_ops_check": ([], i),
             "qi_rope_table": ([i, i, i, vp], i),
             "qi_synth_fill": ([vp, ll, ull, f, f, i, vp], i),
             "qi_ctx_set_hidden_capture": ([vp, vp], i),
@@ -255,6 +264,102 @@ def qkv_norm_rope_i8(act_img, act_txt, w_img, w_txt, norms, pe, nb=1):
                                     _p(w_img[1]), bi, _p(w_txt[0]), _p(w_txt[1]), bt, _p(norms), _p(pe), nb, n_img,
                                     n_txt, _p(out), _stream()))
     return out
+
+
+def _require(ok, what):
+    if not ok:
+        raise QIError(what)
+
+
+def _offsets(seq, device, what):
+    """(begin, end, count) of a sequence argument: int32 offsets of packed
+    sequences [count + 1], or a pair (begin, end) of int32 [count]."""
+    begin, end = seq if isinstance(seq, (tuple, list)) else (seq[:-1], seq[1:])
+    for t in (begin, end):
+        _require(t.dtype == torch.int32 and t.dim() == 1 and t.device == device and t.is_contiguous(),
+                 f"{what}: contiguous int32 offsets on the tensors' device")
+    _require(begin.numel() == end.numel(), f"{what}: begin and end differ in length")
+    return begin, end, begin.numel()
+
+
+def prompt_attention(q, k, v, q_seq, k_seq, max_k, causal=True, scale=None, out=None):
+    """Attention over packed sequences with grouped heads (qi_prompt_attention).
+    q [total_q, heads, head_dim]; k, v [total_k, kv_heads, head_dim]; BF16 or
+    FP16, any strides whose innermost is 1 (views into a fused QKV projection,
+    head-major buffers, cache slabs).  q_seq / k_seq: int32 offsets [batch + 1]
+    of packed sequences, or a pair (begin, end) of int32 [batch].  max_k: the
+    longest key range (a hint).  Returns out [total_q, heads, head_dim]; rows
+    in no query range are left as they were."""
+    _require(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k, v: [rows, heads, head_dim]")
+    dev, dt = q.device, _DT16.get(q.dtype)
+    _require(dt is not None and k.dtype == q.dtype and v.dtype == q.dtype, "q, k, v: all BF16 or all FP16")
+    _require(dev.type == "cuda" and k.device == dev and v.device == dev, "q, k, v: on one GPU")
+    tq, heads, dim = q.shape
+    tk, kv = k.shape[0], k.shape[1]
+    _require(v.shape == k.shape and k.shape[2] == dim, "k, v: same shape, head_dim as q")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    _require(out.shape == q.shape and out.dtype == q.dtype and out.device == dev, "out: as q")
+    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
+    _require(dim == 1 or (qs[2] == ks[2] == vs[2] == os_[2] == 1), "head_dim must be the contiguous dimension")
+    qb, qe, nb = _offsets(q_seq, dev, "q_seq")
+    kb, ke, nk = _offsets(k_seq, dev, "k_seq")
+    _require(nb == nk, "q_seq and k_seq: one entry per sequence")
+    if scale is None:
+        scale = dim ** -0.5
+    L = lib()
+    with torch.cuda.device(dev):
+        nws = L.qi_prompt_attention_workspace(heads, kv, dim, nb, tq, tk, int(max_k))
+        check(-nws if nws < 0 else 0)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+        check(L.qi_prompt_attention(q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
+                                    vs[1], out.data_ptr(), os_[0], os_[1], dt, heads, kv, dim, qb.data_ptr(),
+                                    qe.data_ptr(), kb.data_ptr(), ke.data_ptr(), nb, tq, tk, int(max_k), scale,
+                                    int(causal), ws.data_ptr() if nws else None, nws, _stream()))
+    return out
+
+
+def linear_16bit(x, w, bias=None, act=ACT_NONE, gate=None, residual=None, out_dtype=None, out=None):
+    """residual + gate * act(x w^T + bias) on BF16 / FP16 operands
+    (qi_linear_16bit).  x [M, K], w [N, K] ([2N, K] and bias [2N] for
+    ACT_SWIGLU); gate FP32 [N]; residual and out [M, N] in out_dtype (x's type,
+    or FP32).  residual may be out itself.  Leading dimensions are multiples of
+    16 bytes; the out made here has rows padded to that."""
+    _require(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1], "x [M, K], w [N, K]")
+    dev, dt = x.device, _DT16.get(x.dtype)
+    _require(dt is not None and w.dtype == x.dtype and (bias is None or bias.dtype == x.dtype),
+             "x, w, bias: all BF16 or all FP16")
+    M, K = x.shape
+    wide = 2 if act == ACT_SWIGLU else 1
+    _require(w.shape[0] % wide == 0, "SwiGLU: w holds gate rows and up rows")
+    N = w.shape[0] // wide
+    if out is None:
+        odt = out_dtype or (x.dtype if residual is None else residual.dtype)
+        out = torch.empty(M, -(-N // 8) * 8, dtype=odt, device=dev)[:, :N]
+    _require(out.shape == (M, N) and out.dtype in _DT_OUT and out_dtype in (None, out.dtype), "out: [M, N] in out_dtype")
+    _require(bias is None or (bias.shape == (wide * N,) and bias.is_contiguous()), "bias: [N], contiguous")
+    _require(gate is None or (gate.shape == (N,) and gate.dtype == torch.float32 and gate.is_contiguous()),
+             "gate: FP32 [N], contiguous")
+    _require(residual is None or (residual.shape == (M, N) and residual.dtype == out.dtype), "residual: as out")
+    for t in (x, w, bias, gate, residual, out):
+        _require(t is None or (t.device == dev and dev.type == "cuda"), "all tensors on one GPU")
+    for t in (x, w, residual, out):
+        _require(t is None or t.stride(1) == 1 or t.shape[1] == 1, "rows must be contiguous")
+
+    def ld(t):  # a single row has no leading dimension: any valid one will do
+        return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), -(-t.shape[1] // 8) * 8)
+
+    with torch.cuda.device(dev):
+        check(lib().qi_linear_16bit(x.data_ptr(), ld(x), M, K, w.data_ptr(), ld(w), N, dt, _p(bias), act, _p(gate),
+                                    _p(residual), ld(residual) if residual is not None else 0, out.data_ptr(),
+                                    ld(out), _DT_OUT[out.dtype], _stream()))
+    return out
+
+
+def prompt_ops_check():
+    """Raises QIError if a prompt_attention or linear_16bit call on the current
+    device gave up a bounded wait since the last check; waits for the device."""
+    check(lib().qi_prompt_ops_check())
 
 
 def rope_table(h, w, n_txt):
