@@ -4,13 +4,12 @@
 // with bias, activation, gate and residual applied to the accumulators, so the
 // only traffic is x, w, the residual and the output.
 //
-// Two kernels, chosen by the number of rows M:
-//   * pair kernel (M > kSkinnyRows): CTA pairs, 256 x bn output tiles
-//     (x on the M side), persistent, the epilogue of one tile under the main
-//     loop of the next.  Bound by the tensor cores.
-//   * skinny kernel (M <= kSkinnyRows): the weights on the M side (128 rows of
-//     w per CTA), the x rows as the N side, K split over the CTAs of a
-//     cluster.  Bound by the bytes of w.
+// Two kernels, chosen by the number of rows M of x:
+//   * pair kernel: tcgen05 on CTA pairs, 256 x bn output tiles,
+//     persistent, the epilogue of one tile under the main loop of the next.
+//     Bound by the tensor cores.
+//   * rows kernel (up to 16 rows): w streamed through warp-level MMAs.  Bound by
+//     the bytes of w.
 #include "qi_internal.h"
 #include "sm100.cuh"
 
@@ -21,19 +20,18 @@ namespace {
 
 __device__ int g_linear16_err;  // set by a bounded wait that gave up (linear16_take_error)
 
-constexpr int kSkinnyRows = 128;
 constexpr int BK = 64;  // K elements per pipeline stage: 128 bytes, one swizzle row
 
-struct alignas(64) L16Dev {
-  CUtensorMap tmX, tmW, tmO, tmR;  // x, w; output and residual (pair kernel)
+struct alignas(64) L16Dev {  // pair kernel
+  CUtensorMap tmX, tmW, tmO, tmR;  // x, w, output, residual
   const void* bias;
   const float* gate;
   const void* residual;
   void* out;
   long long ldr, ldo;
   int M, N, K, act;
-  int bn, tiles_m, tiles_n;  // pair kernel
-  int tn, stages, splits;    // skinny kernel
+  int stages;  // TMA pipeline depth
+  int bn, tiles_m, tiles_n;
 };
 
 template <typename T>
@@ -92,7 +90,7 @@ __device__ __forceinline__ void add_bias32(float (&v)[32], const T* p, int n_val
     const uint4* p4 = reinterpret_cast<const uint4*>(p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint4 w = __ldg(p4 + i);
+      const uint4 w = p4[i];
       const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -111,20 +109,17 @@ __device__ __forceinline__ void add_bias32(float (&v)[32], const T* p, int n_val
 // ------------------------------------------------------------------ pair kernel
 namespace pk {
 constexpr int BM = 256, BN_MAX = 256;
-constexpr int A_BYTES = 128 * BK * 2;         // this CTA's 128 rows of x
-constexpr int B_BYTES = BN_MAX / 2 * BK * 2;  // this CTA's half of the tile's w rows
-constexpr int EPI_WARPS = 8;
-constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int A_BYTES = 128 * BK * 2;  // this CTA's 128 rows of x
+constexpr int PROD_WARPS = 2, EPI_WARPS = 8;
+constexpr int THREADS = 32 * (PROD_WARPS + 1 + EPI_WARPS);
 // staging sub-tile of one epilogue warp: 32 rows x 32 columns of the output
 template <typename O>
 constexpr int sub_bytes() { return 32 * 32 * static_cast<int>(sizeof(O)); }
-// 2-byte outputs leave room for a sixth stage
+constexpr int MAX_STAGES = 8;
+constexpr int SMEM_BYTES = 227 * 1024;
+// what the stages may take: narrow tiles get more of them
 template <typename O>
-constexpr int stages() { return sizeof(O) == 4 ? 5 : 6; }
-template <typename O>
-constexpr int smem_bytes() {
-  return 1024 + stages<O>() * (A_BYTES + B_BYTES) + EPI_WARPS * 2 * sub_bytes<O>() + 512;
-}
+constexpr int stage_room() { return SMEM_BYTES - 1024 - 512 - EPI_WARPS * 2 * sub_bytes<O>(); }
 }  // namespace pk
 
 // Tile t of the persistent loop: groups of 8 row blocks, rows fastest within a
@@ -140,15 +135,16 @@ template <typename T, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
     linear16_pair_kernel(const __grid_constant__ L16Dev args) {
   using namespace pk;
-  constexpr int STAGES = stages<O>(), SUB = sub_bytes<O>();
+  constexpr int SUB = sub_bytes<O>();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stages = args.stages, b_bytes = args.bn / 2 * BK * 2;  // b: this CTA's half of the tile's w rows
   uint8_t* sA = smem;
-  uint8_t* sB = smem + STAGES * A_BYTES;
-  uint8_t* sE = sB + STAGES * B_BYTES;
+  uint8_t* sB = smem + stages * A_BYTES;
+  uint8_t* sE = sB + stages * b_bytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(sE + EPI_WARPS * 2 * SUB);
-  uint64_t* empty = full + STAGES;
-  uint64_t* tfull = empty + STAGES;
+  uint64_t* empty = full + MAX_STAGES;
+  uint64_t* tfull = empty + MAX_STAGES;
   uint64_t* tempty = tfull + 2;
   uint64_t* xfull = tempty + 2;  // [EPI_WARPS][2] residual sub-tile loaded
   uint64_t* drain = xfull + 2 * EPI_WARPS;
@@ -165,7 +161,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
   const int kblocks = (args.K + BK - 1) / BK;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -182,7 +178,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
     tma_prefetch_desc(&args.tmO);
     if (args.residual) tma_prefetch_desc(&args.tmR);
   }
-  if (warp == 1) {
+  if (warp == PROD_WARPS) {
     tmem_alloc_pair(tmem_slot, 512);
     tmem_relinquish_pair();
   }
@@ -191,12 +187,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
   cluster_sync();  // both CTAs' barriers exist before either signals the other
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  grid_dependency_wait();
+  launch_dependents();
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer (both CTAs)
+  if (warp < PROD_WARPS) {
+    // ------------------------------------------------------------ producers (both CTAs)
+    // Warp 0 brings x, warp 1 brings w: waiting for a stage and issuing both
+    // copies takes one thread ~430 clocks, more than a narrow tile's MMAs.
     if (lane == 0) {
       const uint32_t full0 = mapa_shared(&full[0], 0);  // the even CTA's stage barriers
-      const uint32_t stage_tx = 2 * (A_BYTES + bn / 2 * BK * 2);  // both CTAs' bytes
+      const uint32_t stage_tx = 2 * (A_BYTES + b_bytes);  // both CTAs' bytes
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -206,16 +206,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
         // SwiGLU: the even CTA brings the tile's gate rows of w, the odd CTA
         // its up rows, so accumulator columns [0, bn/2) are the gate products
         const int wrow = wide ? nt * bn_out + static_cast<int>(cr) * args.N : nt * bn + (bn / 2) * static_cast<int>(cr);
+        const int row = warp == 0 ? m0 + 128 * static_cast<int>(cr) : wrow;
+        const CUtensorMap* tm = warp == 0 ? &args.tmX : &args.tmW;
+        uint8_t* dst = warp == 0 ? sA : sB;
+        const int bytes = warp == 0 ? A_BYTES : b_bytes;
         for (int kb = 0; kb < kblocks; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag)) {
             ok = false;
             break;
           }
-          if (leader) mbar_expect_tx(&full[stage], stage_tx);
-          const uint32_t fb = full0 + stage * 8;
-          tma_load_2d_pair(sA + stage * A_BYTES, &args.tmX, kb * BK, m0 + 128 * static_cast<int>(cr), fb);
-          tma_load_2d_pair(sB + stage * B_BYTES, &args.tmW, kb * BK, wrow, fb);
-          if (++stage == STAGES) {
+          if (leader && warp == 0) mbar_expect_tx(&full[stage], stage_tx);
+          tma_load_2d_pair(dst + stage * bytes, tm, kb * BK, row, full0 + stage * 8);
+          if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
@@ -231,7 +233,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
         }
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == PROD_WARPS) {
     // ------------------------------------------------------------ MMA issuer (even CTA)
     if (leader) {
       auto wait_all = [&](uint64_t* bar, uint32_t parity) {
@@ -239,7 +241,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
       };
       int stage = 0, local = 0;
       uint32_t phase = 0;
-      bool ok = true;
+      bool ok = true, ready = mbar_test_wait(&full[0], 0);
       const uint32_t idesc = idesc16<T>(BM, 0) | (static_cast<uint32_t>(bn >> 3) << 17);
       const uint64_t ad0 = umma_desc_sw128(smem_u32(sA), 16, 1024), bd0 = umma_desc_sw128(smem_u32(sB), 16, 1024);
       for (int t = cluster; t < total && ok; t += nclusters, ++local) {
@@ -251,21 +253,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * BN_MAX;
         for (int kb = 0; kb < kblocks; ++kb) {
-          if (!wait_all(&full[stage], phase)) {
+          if (!__all_sync(0xffffffffu, ready) && !wait_all(&full[stage], phase)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint64_t ad = ad0 + static_cast<uint64_t>((stage * A_BYTES) >> 4);
-          const uint64_t bd = bd0 + static_cast<uint64_t>((stage * B_BYTES) >> 4);
-#pragma unroll
-          for (int k = 0; k < BK / 16; ++k)
-            mma_f16_ss_pair_elect(d_tmem, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
-          mma_commit_pair_elect(&empty[stage], 0x3);
-          if (++stage == STAGES) {
+          const int cur = stage;
+          if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
+          ready = mbar_test_wait(&full[stage], phase);
+          const uint64_t ad = ad0 + static_cast<uint64_t>((cur * A_BYTES) >> 4);
+          const uint64_t bd = bd0 + static_cast<uint64_t>((cur * b_bytes) >> 4);
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k)
+            mma_f16_ss_pair_elect(d_tmem, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+          mma_commit_pair_elect(&empty[cur], 0x3);
         }
         if (!ok) break;
         mma_commit_pair_elect(&tfull[buf], 0x3);
@@ -289,7 +293,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
     // residual, if any) -> TMA store, which clips rows and columns past the
     // end.  Two staging buffers per warp; the next chunk's residual is loaded
     // into the free one meanwhile.
-    const int quarter = warp & 3, ew = warp - 2, half = ew >> 2;
+    const int quarter = warp & 3, ew = warp - PROD_WARPS - 1, half = ew >> 2;
     uint8_t* ebuf = sE + ew * 2 * SUB;
     uint64_t* xb = xfull + ew * 2;
     const uint32_t tempty0 = mapa_shared(&tempty[0], 0);
@@ -370,7 +374,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
             const float4* g4 = reinterpret_cast<const float4*>(args.gate + col);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const float4 g = __ldg(g4 + j);
+              const float4 g = g4[j];
               v[4 * j] *= g.x;
               v[4 * j + 1] *= g.y;
               v[4 * j + 2] *= g.z;
@@ -445,221 +449,161 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // both CTAs finished with TMEM and each other's barriers
-  if (warp == 1) {
+  if (warp == PROD_WARPS) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 512);
   }
 }
 
-// ------------------------------------------------------------------ skinny kernel
-// One CTA: 128 rows of w (for SwiGLU 128 gate and 128 up rows) against all of
-// x's rows (padded to tn, the MMA's N), over its share of K.  The accumulator's
-// TMEM lanes are output columns, so a warp writes 32 neighbouring columns of a
-// row at once.  The CTAs of a cluster hold the partial sums of the K splits:
-// each puts them into its shared memory as [row][128], and CTA r adds up rows
-// r, r + splits, ... over the cluster (in split order: the sum does not depend
-// on timing) and runs the epilogue on them.
-namespace sk {
-constexpr int W_BYTES = 128 * BK * 2;
-constexpr int THREADS = 192;
-}  // namespace sk
+// ------------------------------------------------------------------ rows kernel
+// Few rows of x: the bytes of w are what counts, so w goes from HBM straight to
+// the registers of warp-level MMAs (m16n8k16: 16 rows of w, 8 rows of x), every
+// load 16 bytes per thread and several in flight, with no staging to wait for.
+// The K index of an MMA is a summation index, so its order is free: a thread's
+// 16 bytes (8 neighbouring k) are taken as its slots of two MMAs, for w and x
+// alike.  A CTA makes 16 columns (SwiGLU: 16 gate and 16 up rows of w); its 8
+// warps take 32-k blocks of K in turn and add up in shared memory, in warp
+// order.  One row, N = K = 3584 (25.7 MB of w): 9.8 us; a kernel that only reads
+// those bytes takes 8.1-8.7 us from launch to launch.
+namespace rk {
+constexpr int WARPS = 8, THREADS = 32 * WARPS;
+constexpr int UNROLL = 4;  // 32-k blocks whose loads are in flight per warp
+}  // namespace rk
 
-template <typename T, typename O, bool WIDE>
-__global__ void __launch_bounds__(sk::THREADS) linear16_skinny_kernel(const __grid_constant__ L16Dev args) {
-  using namespace sk;
-  constexpr int NW = WIDE ? 2 : 1;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int tn = args.tn, stages = args.stages, splits = args.splits;
-  const int x_bytes = tn * BK * 2, stage_bytes = NW * W_BYTES + x_bytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + stages * stage_bytes);
-  uint64_t* empty = full + stages;
-  uint64_t* done = empty + stages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+template <typename T>
+__device__ __forceinline__ void mma_m16n8k16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+  if (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = blockIdx.x % splits, n0 = (blockIdx.x / splits) * 128;
-  const int kblocks = (args.K + BK - 1) / BK;
-  const int kb0 = static_cast<int>(static_cast<long long>(kblocks) * rank / splits);
-  const int kb1 = static_cast<int>(static_cast<long long>(kblocks) * (rank + 1) / splits);
-  const uint32_t cols = NW * tn < 32 ? 32 : NW * tn;  // TMEM columns: a power of two
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    mbar_init(done, 1);
-    *abort_flag = 0;
-    fence_mbar_init();
-    tma_prefetch_desc(&args.tmX);
-    tma_prefetch_desc(&args.tmW);
+// Eight neighbouring k of a row from k on, zeros from K on.
+template <typename T, bool STREAM>
+__device__ __forceinline__ uint4 load8(const T* row, int k, int K) {
+  if (k + 8 <= K) {
+    uint4 v;
+    if (STREAM)
+      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                   : "l"(row + k));
+    else
+      v = *reinterpret_cast<const uint4*>(row + k);
+    return v;
   }
-  if (warp == 1) {
-    tmem_alloc(tmem_slot, cols);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  bool ok = true;
-
-  if (warp == 0) {
-    if (lane == 0) {
-      const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
-      int stage = 0, last = -1;
-      uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag)) {
-          ok = false;
-          break;
-        }
-        uint8_t* st = smem + stage * stage_bytes;
-        mbar_expect_tx(&full[stage], stage_bytes);
-        tma_load_2d_hint(st, &args.tmW, kb * BK, n0, &full[stage], pol_w);
-        if (WIDE) tma_load_2d_hint(st + W_BYTES, &args.tmW, kb * BK, args.N + n0, &full[stage], pol_w);
-        tma_load_2d_hint(st + NW * W_BYTES, &args.tmX, kb * BK, 0, &full[stage], pol_x);
-        last = kb - kb0;
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-      if (!ok) {
-        *abort_flag = 1;
-        atomicCAS(&g_linear16_err, 0, kErrTimeoutProducer);
-        // copies already issued land before the CTA exits
-        for (int i = last < stages ? 0 : last - stages + 1; i <= last; ++i) {
-          const uint64_t t0 = global_timer_ns();
-          while (!mbar_try_wait(&full[i % stages], (i / stages) & 1) && global_timer_ns() - t0 < kWaitLimitNs / 4) {
-          }
-        }
-      }
-    }
-  } else if (warp == 1) {
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
-    };
-    const uint32_t idesc = idesc16<T>(128, 0) | (static_cast<uint32_t>(tn >> 3) << 17);
-    const uint64_t d0 = umma_desc_sw128(smem_u32(smem), 16, 1024);
-    int stage = 0;
-    uint32_t phase = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      if (!wait_all(&full[stage], phase)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      const uint64_t wd = d0 + static_cast<uint64_t>((stage * stage_bytes) >> 4);
-      const uint64_t xd = wd + static_cast<uint64_t>((NW * W_BYTES) >> 4);
+  uint32_t u[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int k = 0; k < BK / 16; ++k) {
-        const uint32_t more = kb > kb0 || k > 0 ? 1u : 0u;
-        mma_f16_ss_elect(tmem_base, wd + 2 * k, xd + 2 * k, idesc, more);
-        if (WIDE)
-          mma_f16_ss_elect(tmem_base + tn, wd + (W_BYTES >> 4) + 2 * k, xd + 2 * k, idesc, more);
-      }
-      mma_commit_elect(&empty[stage]);
-      if (++stage == stages) {
-        stage = 0;
-        phase ^= 1u;
-      }
+  for (int e = 0; e < 8; ++e)
+    if (k + e < K) u[e >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[k + e]) << (16 * (e & 1));
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+// G: groups of 8 rows of x; R: 16-row tiles of w per warp (SwiGLU: gate, up).
+template <typename T, typename O, int G, int R, bool WIDE>
+__global__ void __launch_bounds__(rk::THREADS) linear16_rows_kernel(const __grid_constant__ Linear16Args args) {
+  using namespace rk;
+  constexpr int COLS = WIDE ? 16 : 16 * R;               // output columns of the CTA
+  constexpr int STRIDE = 16 * R + 4;                     // floats per x row in shared memory: conflict-free stores
+  constexpr int SWEEPS = (8 * G * COLS + THREADS - 1) / THREADS;
+  extern __shared__ float red[];                         // [WARPS][8 G][STRIDE]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * COLS;
+  const long long last = (WIDE ? 2ll : 1ll) * args.N - 1;
+  const T* wrow[R][2];  // rows g and g + 8 of each tile; past the end the last row, whose sums nobody reads
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      long long n = n0 + g + 8 * h + (WIDE ? static_cast<long long>(r) * args.N : 16 * r);
+      if (n > last) n = last;
+      wrow[r][h] = static_cast<const T*>(args.w) + n * args.ldw;
     }
-    if (!ok && lane == 0) {
-      *abort_flag = 1;
-      atomicCAS(&g_linear16_err, 0, kErrTimeoutMma);
-    }
-    __syncwarp();
-    mma_commit_elect(done);  // also before teardown after a failed wait
-    const uint64_t t0 = global_timer_ns();
-    while (!mbar_try_wait(done, 0) && global_timer_ns() - t0 < kWaitLimitNs / 4) {
+  const T* xrow[G];
+#pragma unroll
+  for (int j = 0; j < G; ++j) xrow[j] = static_cast<const T*>(args.x) + min(8 * j + g, args.M - 1) * args.ldx;
+  grid_dependency_wait();
+  launch_dependents();
+
+  // this thread's outputs: column n0 + c, rows m0, m0 + THREADS / COLS, ...
+  const int c = threadIdx.x % COLS, m0 = threadIdx.x / COLS, col = n0 + c;
+  const bool in = col < args.N;
+  float bias0 = 0.0f, bias1 = 0.0f, gate = 1.0f;
+  O res[SWEEPS];
+  if (in) {
+    const T* bias = static_cast<const T*>(args.bias);
+    if (bias) bias0 = cvt_in(bias[col]);
+    if (WIDE && bias) bias1 = cvt_in(bias[args.N + col]);
+    if (args.gate) gate = args.gate[col];
+    if (args.residual) {
+#pragma unroll
+      for (int i = 0; i < SWEEPS; ++i) {
+        const long long m = m0 + i * (THREADS / COLS);
+        if (m < args.M) res[i] = static_cast<const O*>(args.residual)[m * args.ldr + col];
+      }
     }
   }
 
-  // epilogue warps: thread = output column (TMEM lane)
-  const int quarter = warp & 3, lcol = quarter * 32 + lane, col = n0 + lcol;
-  const uint32_t trow = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-  float bias0 = 0.0f, bias1 = 0.0f, gate = 1.0f;
-  const bool in = col < args.N;
-  if (warp >= 2 && in) {
-    const T* bias = static_cast<const T*>(args.bias);
-    if (bias) {
-      bias0 = cvt_in(bias[col]);
-      if (WIDE) bias1 = cvt_in(bias[args.N + col]);
+  float acc[R][G][4] = {};
+  const int kblocks = (args.K + 31) / 32;
+#pragma unroll 1
+  for (int kb = warp; kb < kblocks; kb += WARPS * UNROLL) {
+    uint4 w[UNROLL][R][2];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int k = (kb + u * WARPS) * 32 + 8 * t;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        w[u][r][0] = load8<T, true>(wrow[r][0], k, args.K);
+        w[u][r][1] = load8<T, true>(wrow[r][1], k, args.K);
+      }
     }
-    if (args.gate) gate = args.gate[col];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int k = (kb + u * WARPS) * 32 + 8 * t;
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        const uint4 x = load8<T, false>(xrow[j], k, args.K);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          mma_m16n8k16<T>(acc[r][j], w[u][r][0].x, w[u][r][1].x, w[u][r][0].y, w[u][r][1].y, x.x, x.y);
+          mma_m16n8k16<T>(acc[r][j], w[u][r][0].z, w[u][r][1].z, w[u][r][0].w, w[u][r][1].w, x.z, x.w);
+        }
+      }
+    }
   }
-  // one output element from its sum(s)
-  auto finish = [&](int m, float v, float u) {
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        red[(warp * 8 * G + 8 * j + 2 * t + (e & 1)) * STRIDE + 16 * r + g + 8 * (e >> 1)] = acc[r][j][e];
+  __syncthreads();
+  if (!in) return;
+#pragma unroll
+  for (int i = 0; i < SWEEPS; ++i) {
+    const int m = m0 + i * (THREADS / COLS);
+    if (m >= args.M) break;
+    float v = 0.0f, u = 0.0f;
+#pragma unroll
+    for (int q = 0; q < WARPS; ++q) {
+      const float* p = red + (q * 8 * G + m) * STRIDE + c;
+      v += p[0];
+      if (WIDE) u += p[16];
+    }
     v += bias0;
     if (WIDE)
       v = v * sigmoid_f32(v) * (u + bias1);
     else
       v = activate(v, args.act);
     v *= gate;
-    if (args.residual) v += cvt_in(static_cast<const O*>(args.residual)[m * args.ldr + col]);
+    if (args.residual) v += cvt_in(res[i]);
     static_cast<O*>(args.out)[m * args.ldo + col] = cvt_out<O>(v);
-  };
-  float* part = reinterpret_cast<float*>(smem);  // [NW][M][128] partial sums, over the consumed stages
-  if (warp >= 2) {
-    const bool w = mbar_wait(done, 0, abort_flag);
-    ok = __all_sync(0xffffffffu, w && !*abort_flag);
-    if (!ok && lane == 0) {
-      *abort_flag = 1;
-      atomicCAS(&g_linear16_err, 0, kErrTimeoutEpilogue);
-    }
-    tc_fence_after();
-    if (ok) {
-#pragma unroll 1
-      for (int c = 0; c < args.M; c += 16) {
-        uint32_t r[16], r2[16];
-        tmem_ld16(trow + c, r);
-        if (WIDE) tmem_ld16(trow + tn + c, r2);
-        tmem_ld_wait();
-        tmem_reg_fence16(r);
-        if (WIDE) tmem_reg_fence16(r2);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (c + j >= args.M) break;
-          if (splits == 1) {
-            if (in) finish(c + j, __uint_as_float(r[j]), WIDE ? __uint_as_float(r2[j]) : 0.0f);
-          } else {
-            part[(c + j) * 128 + lcol] = __uint_as_float(r[j]);
-            if (WIDE) part[(args.M + c + j) * 128 + lcol] = __uint_as_float(r2[j]);
-          }
-        }
-      }
-    }
-  }
-  if (splits > 1) {
-    __syncthreads();
-    cluster_sync();
-    if (warp >= 2 && in && ok) {
-      uint32_t base[8];
-#pragma unroll
-      for (int s = 0; s < 8; ++s) base[s] = s < splits ? mapa_shared(part, s) + lcol * 4 : 0u;
-#pragma unroll 1
-      for (int m = rank; m < args.M; m += splits) {
-        float v = 0.0f, u = 0.0f;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          if (s >= splits) break;
-          v += ld_cluster_f32(base[s] + m * 512);
-          if (WIDE) u += ld_cluster_f32(base[s] + (args.M + m) * 512);
-        }
-        finish(m, v, u);
-      }
-    }
-    __syncwarp();
-    cluster_sync();  // nobody leaves while its sums are being read
-  }
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem_base, cols);
   }
 }
 
@@ -684,6 +628,12 @@ int encode(CUtensorMap* tm, const void* base, long long rows, long long cols, lo
   return r == CUDA_SUCCESS ? QI_OK : QI_ERR_CUDA;
 }
 
+// An operand [rows, K], K tail filled with zeros: boxes of one atom.
+template <typename T>
+int encode_operand(CUtensorMap* tm, const void* base, long long rows, int K, long long ld, int box_rows) {
+  return encode<T>(tm, base, rows, K, ld, BK, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 // Pair-tile width: the one whose waves over the SM pairs, times the tile's
 // time, finish first.
 int pair_width(int M, int cols, bool wide, int clusters) {
@@ -700,6 +650,22 @@ int pair_width(int M, int cols, bool wide, int clusters) {
   return best;
 }
 
+// Launch with the dependent-launch attribute (see grid_dependency_wait).
+template <typename A>
+int launch16(void (*fn)(const A), unsigned grid, int threads, int smem, const A& args, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fn, args) == cudaSuccess ? QI_OK : QI_ERR_CUDA;
+}
+
 template <typename T, typename O>
 int launch_pair16(const Linear16Args& a, L16Dev& d, cudaStream_t stream, int num_sms) {
   const bool wide = a.act == QI_ACT_SWIGLU;
@@ -709,57 +675,42 @@ int launch_pair16(const Linear16Args& a, L16Dev& d, cudaStream_t stream, int num
   d.tiles_m = (a.M + pk::BM - 1) / pk::BM;
   d.tiles_n = (a.N + bn_out - 1) / bn_out;
   if (static_cast<long long>(d.tiles_m) * d.tiles_n > 0x7fffffff) return QI_ERR_UNSUPPORTED;
+  d.stages = pk::stage_room<O>() / (pk::A_BYTES + d.bn / 2 * BK * 2);
+  if (d.stages > pk::MAX_STAGES) d.stages = pk::MAX_STAGES;
   const CUtensorMapSwizzle osw = sizeof(O) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
-  if (encode<T>(&d.tmX, a.x, a.M, a.K, a.ldx, BK, 128, CU_TENSOR_MAP_SWIZZLE_128B) != QI_OK ||
-      encode<T>(&d.tmW, a.w, (wide ? 2ll : 1ll) * a.N, a.K, a.ldw, BK, d.bn / 2, CU_TENSOR_MAP_SWIZZLE_128B) != QI_OK ||
+  if (encode_operand<T>(&d.tmX, a.x, a.M, a.K, a.ldx, 128) != QI_OK ||
+      encode_operand<T>(&d.tmW, a.w, (wide ? 2ll : 1ll) * a.N, a.K, a.ldw, d.bn / 2) != QI_OK ||
       encode<O>(&d.tmO, a.out, a.M, a.N, a.ldo, 32, 32, osw) != QI_OK ||
       (a.residual && encode<O>(&d.tmR, a.residual, a.M, a.N, a.ldr, 32, 32, osw) != QI_OK))
     return QI_ERR_CUDA;
   static unsigned long long attr_done = 0;
   const auto fn = linear16_pair_kernel<T, O>;
-  if (smem_optin(reinterpret_cast<const void*>(fn), pk::smem_bytes<O>(), &attr_done) != QI_OK) return QI_ERR_CUDA;
+  if (smem_optin(reinterpret_cast<const void*>(fn), pk::SMEM_BYTES, &attr_done) != QI_OK) return QI_ERR_CUDA;
   const int tiles = d.tiles_m * d.tiles_n;
-  fn<<<2 * (tiles < clusters ? tiles : clusters), pk::THREADS, pk::smem_bytes<O>(), stream>>>(d);
-  return cudaGetLastError() == cudaSuccess ? QI_OK : QI_ERR_CUDA;
+  return launch16(fn, 2u * (tiles < clusters ? tiles : clusters), pk::THREADS, pk::SMEM_BYTES, d, stream);
 }
 
-template <typename T, typename O, bool WIDE>
-int launch_skinny(const Linear16Args& a, L16Dev& d, cudaStream_t stream, int num_sms) {
-  constexpr int NW = WIDE ? 2 : 1;
-  d.tn = a.M <= 16 ? 16 : (a.M <= 32 ? 32 : (a.M <= 64 ? 64 : 128));
-  const int tiles = (a.N + 127) / 128, kblocks = (a.K + BK - 1) / BK;
-  // K splits: about one CTA per SM, at least four K blocks each
-  int splits = (num_sms - 8 + tiles - 1) / tiles;
-  if (splits > kblocks / 4) splits = kblocks / 4;
-  d.splits = splits < 1 ? 1 : (splits > 8 ? 8 : splits);
-  // stages: two CTAs per SM where three or more of them fit, else one
-  const int stage = NW * sk::W_BYTES + d.tn * BK * 2;
-  d.stages = (110 * 1024) / stage;
-  if (d.stages < 3) d.stages = (220 * 1024) / stage;
-  if (d.stages > 8) d.stages = 8;
-  const int smem = 1024 + d.stages * stage + 256;
-  if (encode<T>(&d.tmX, a.x, a.M, a.K, a.ldx, BK, d.tn, CU_TENSOR_MAP_SWIZZLE_128B) != QI_OK ||
-      encode<T>(&d.tmW, a.w, static_cast<long long>(NW) * a.N, a.K, a.ldw, BK, 128, CU_TENSOR_MAP_SWIZZLE_128B) != QI_OK)
-    return QI_ERR_CUDA;
+template <typename T, typename O, int G, int R, bool WIDE>
+int launch_rows(const Linear16Args& a, cudaStream_t stream) {
+  constexpr int COLS = WIDE ? 16 : 16 * R;
+  constexpr int smem = rk::WARPS * 8 * G * (16 * R + 4) * 4;
   static unsigned long long attr_done = 0;
-  const auto fn = linear16_skinny_kernel<T, O, WIDE>;
-  if (smem_optin(reinterpret_cast<const void*>(fn), 222 * 1024, &attr_done) != QI_OK) return QI_ERR_CUDA;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles) * d.splits);
-  cfg.blockDim = dim3(sk::THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = d.splits;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fn, static_cast<const L16Dev&>(d)) == cudaSuccess ? QI_OK : QI_ERR_CUDA;
+  const auto fn = linear16_rows_kernel<T, O, G, R, WIDE>;
+  if (smem > 48 * 1024 && smem_optin(reinterpret_cast<const void*>(fn), smem, &attr_done) != QI_OK) return QI_ERR_CUDA;
+  return launch16(fn, static_cast<unsigned>((a.N + COLS - 1) / COLS), rk::THREADS, smem, a, stream);
 }
 
 template <typename T, typename O>
 int launch_typed(const Linear16Args& a, cudaStream_t stream) {
+  // The rows kernel where it is the faster one (us, rows / pair kernel, FP32 or
+  // 16-bit out): N 4608, K 3584: 1 row 10.4 / 16.7, 16 rows 14.0 / 16.8, 24 rows
+  // 18.8 / 15.6; N = K = 512: 1 row 2.6 / 4.9; SwiGLU, N 14336, K 3584: 1 row
+  // 45 / 46, 8 rows 50 / 46 (but 2.6 / 4.9 at small sizes), 16 rows 62 / 46.
+  if (a.act == QI_ACT_SWIGLU) {
+    if (a.M <= 8) return launch_rows<T, O, 1, 2, true>(a, stream);
+  } else if (a.M <= 16) {
+    return a.M <= 8 ? launch_rows<T, O, 1, 1, false>(a, stream) : launch_rows<T, O, 2, 1, false>(a, stream);
+  }
   L16Dev d;
   memset(&d, 0, sizeof(d));
   d.bias = a.bias;
@@ -772,10 +723,7 @@ int launch_typed(const Linear16Args& a, cudaStream_t stream) {
   d.N = a.N;
   d.K = a.K;
   d.act = a.act;
-  const int num_sms = device_num_sms();
-  if (a.M > kSkinnyRows) return launch_pair16<T, O>(a, d, stream, num_sms);
-  return a.act == QI_ACT_SWIGLU ? launch_skinny<T, O, true>(a, d, stream, num_sms)
-                                : launch_skinny<T, O, false>(a, d, stream, num_sms);
+  return launch_pair16<T, O>(a, d, stream, device_num_sms());
 }
 
 }  // namespace

@@ -266,20 +266,29 @@ def qkv_norm_rope_i8(act_img, act_txt, w_img, w_txt, norms, pe, nb=1):
     return out
 
 
-def _require(ok, what):
-    if not ok:
-        raise QIError(what)
+def _on_device(t):
+    """Index of the GPU that holds t, and a guard that makes it current (None
+    when it is already)."""
+    dev = t.device
+    if dev.type != "cuda":
+        raise QIError("tensors must be on a GPU")
+    return dev.index, None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev.index)
 
 
-def _offsets(seq, device, what):
-    """(begin, end, count) of a sequence argument: int32 offsets of packed
-    sequences [count + 1], or a pair (begin, end) of int32 [count]."""
-    begin, end = seq if isinstance(seq, (tuple, list)) else (seq[:-1], seq[1:])
-    for t in (begin, end):
-        _require(t.dtype == torch.int32 and t.dim() == 1 and t.device == device and t.is_contiguous(),
-                 f"{what}: contiguous int32 offsets on the tensors' device")
-    _require(begin.numel() == end.numel(), f"{what}: begin and end differ in length")
-    return begin, end, begin.numel()
+def _offsets(seq, index, what):
+    """(begin pointer, end pointer, count) of a sequence argument: int32 offsets
+    of packed sequences [count + 1], or a pair (begin, end) of int32 [count]."""
+    pair = isinstance(seq, (tuple, list))
+    for t in seq if pair else (seq,):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.get_device() != index or not t.is_contiguous():
+            raise QIError(f"{what}: contiguous int32 offsets on the tensors' GPU")
+    if pair:
+        if len(seq) != 2 or seq[0].numel() != seq[1].numel():
+            raise QIError(f"{what}: begin and end differ in length")
+        return seq[0].data_ptr(), seq[1].data_ptr(), seq[0].numel()
+    if seq.numel() < 1:
+        raise QIError(f"{what}: one more offset than sequences")
+    return seq.data_ptr(), seq.data_ptr() + 4, seq.numel() - 1
 
 
 def prompt_attention(q, k, v, q_seq, k_seq, max_k, causal=True, scale=None, out=None):
@@ -289,33 +298,45 @@ def prompt_attention(q, k, v, q_seq, k_seq, max_k, causal=True, scale=None, out=
     head-major buffers, cache slabs).  q_seq / k_seq: int32 offsets [batch + 1]
     of packed sequences, or a pair (begin, end) of int32 [batch].  max_k: the
     longest key range (a hint).  Returns out [total_q, heads, head_dim]; rows
-    in no query range are left as they were."""
-    _require(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k, v: [rows, heads, head_dim]")
-    dev, dt = q.device, _DT16.get(q.dtype)
-    _require(dt is not None and k.dtype == q.dtype and v.dtype == q.dtype, "q, k, v: all BF16 or all FP16")
-    _require(dev.type == "cuda" and k.device == dev and v.device == dev, "q, k, v: on one GPU")
+    in no query range are left as they were.  Runs on the tensors' GPU, on its
+    current stream."""
+    if not (q.dim() == k.dim() == v.dim() == 3):
+        raise QIError("q, k, v: [rows, heads, head_dim]")
+    dt = _DT16.get(q.dtype)
+    if dt is None or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise QIError("q, k, v: all BF16 or all FP16")
+    index, guard = _on_device(q)
     tq, heads, dim = q.shape
-    tk, kv = k.shape[0], k.shape[1]
-    _require(v.shape == k.shape and k.shape[2] == dim, "k, v: same shape, head_dim as q")
+    tk, kv, kdim = k.shape
+    if v.shape != k.shape or kdim != dim:
+        raise QIError("k, v: same shape, head_dim as q")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    _require(out.shape == q.shape and out.dtype == q.dtype and out.device == dev, "out: as q")
-    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
-    _require(dim == 1 or (qs[2] == ks[2] == vs[2] == os_[2] == 1), "head_dim must be the contiguous dimension")
-    qb, qe, nb = _offsets(q_seq, dev, "q_seq")
-    kb, ke, nk = _offsets(k_seq, dev, "k_seq")
-    _require(nb == nk, "q_seq and k_seq: one entry per sequence")
-    if scale is None:
-        scale = dim ** -0.5
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise QIError("out: as q")
+    if not (k.get_device() == v.get_device() == out.get_device() == index):
+        raise QIError("q, k, v, out: on one GPU")
+    (q0, q1, q2), (k0, k1, k2), (v0, v1, v2), (o0, o1, o2) = q.stride(), k.stride(), v.stride(), out.stride()
+    if not (q2 == k2 == v2 == o2 == 1):
+        raise QIError("head_dim must be the contiguous dimension")
+    qb, qe, nb = _offsets(q_seq, index, "q_seq")
+    kb, ke, nk = _offsets(k_seq, index, "k_seq")
+    if nb != nk:
+        raise QIError("q_seq and k_seq: one entry per sequence")
+    if guard is not None:
+        with guard:
+            return prompt_attention(q, k, v, q_seq, k_seq, max_k, causal, scale, out)
     L = lib()
-    with torch.cuda.device(dev):
-        nws = L.qi_prompt_attention_workspace(heads, kv, dim, nb, tq, tk, int(max_k))
+    nws = L.qi_prompt_attention_workspace(heads, kv, dim, nb, tq, tk, max_k)
+    if nws:
         check(-nws if nws < 0 else 0)
-        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-        check(L.qi_prompt_attention(q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
-                                    vs[1], out.data_ptr(), os_[0], os_[1], dt, heads, kv, dim, qb.data_ptr(),
-                                    qe.data_ptr(), kb.data_ptr(), ke.data_ptr(), nb, tq, tk, int(max_k), scale,
-                                    int(causal), ws.data_ptr() if nws else None, nws, _stream()))
+        ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
+    st = L.qi_prompt_attention(q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, out.data_ptr(), o0, o1, dt,
+                               heads, kv, dim, qb, qe, kb, ke, nb, tq, tk, max_k, dim ** -0.5 if scale is None else scale,
+                               1 if causal else 0, ws.data_ptr() if nws else None, nws,
+                               torch._C._cuda_getCurrentRawStream(index))
+    if st:
+        check(st)
     return out
 
 
@@ -324,35 +345,65 @@ def linear_16bit(x, w, bias=None, act=ACT_NONE, gate=None, residual=None, out_dt
     (qi_linear_16bit).  x [M, K], w [N, K] ([2N, K] and bias [2N] for
     ACT_SWIGLU); gate FP32 [N]; residual and out [M, N] in out_dtype (x's type,
     or FP32).  residual may be out itself.  Leading dimensions are multiples of
-    16 bytes; the out made here has rows padded to that."""
-    _require(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1], "x [M, K], w [N, K]")
-    dev, dt = x.device, _DT16.get(x.dtype)
-    _require(dt is not None and w.dtype == x.dtype and (bias is None or bias.dtype == x.dtype),
-             "x, w, bias: all BF16 or all FP16")
-    M, K = x.shape
+    16 bytes; the out made here has rows padded to that.  Runs on the tensors'
+    GPU, on its current stream."""
+    if not x.dim() == w.dim() == 2:
+        raise QIError("x [M, K], w [N, K]")
+    (M, K), (rows, kw) = x.shape, w.shape
+    xdt = x.dtype
+    dt = _DT16.get(xdt)
+    if dt is None or w.dtype != xdt:
+        raise QIError("x, w: all BF16 or all FP16")
     wide = 2 if act == ACT_SWIGLU else 1
-    _require(w.shape[0] % wide == 0, "SwiGLU: w holds gate rows and up rows")
-    N = w.shape[0] // wide
+    N = rows // wide
+    if kw != K or N * wide != rows:
+        raise QIError("w [N, K]; for SwiGLU N gate rows, then N up rows")
+    index, guard = _on_device(x)
     if out is None:
-        odt = out_dtype or (x.dtype if residual is None else residual.dtype)
-        out = torch.empty(M, -(-N // 8) * 8, dtype=odt, device=dev)[:, :N]
-    _require(out.shape == (M, N) and out.dtype in _DT_OUT and out_dtype in (None, out.dtype), "out: [M, N] in out_dtype")
-    _require(bias is None or (bias.shape == (wide * N,) and bias.is_contiguous()), "bias: [N], contiguous")
-    _require(gate is None or (gate.shape == (N,) and gate.dtype == torch.float32 and gate.is_contiguous()),
-             "gate: FP32 [N], contiguous")
-    _require(residual is None or (residual.shape == (M, N) and residual.dtype == out.dtype), "residual: as out")
-    for t in (x, w, bias, gate, residual, out):
-        _require(t is None or (t.device == dev and dev.type == "cuda"), "all tensors on one GPU")
-    for t in (x, w, residual, out):
-        _require(t is None or t.stride(1) == 1 or t.shape[1] == 1, "rows must be contiguous")
-
-    def ld(t):  # a single row has no leading dimension: any valid one will do
-        return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), -(-t.shape[1] // 8) * 8)
-
-    with torch.cuda.device(dev):
-        check(lib().qi_linear_16bit(x.data_ptr(), ld(x), M, K, w.data_ptr(), ld(w), N, dt, _p(bias), act, _p(gate),
-                                    _p(residual), ld(residual) if residual is not None else 0, out.data_ptr(),
-                                    ld(out), _DT_OUT[out.dtype], _stream()))
+        odt = out_dtype or (xdt if residual is None else residual.dtype)
+        out = torch.empty((M, N), dtype=odt, device=x.device) if N % 8 == 0 else torch.empty(
+            (M, -(-N // 8) * 8), dtype=odt, device=x.device)[:, :N]
+    elif out.shape != (M, N) or (out_dtype is not None and out.dtype != out_dtype):
+        raise QIError("out: [M, N] in out_dtype")
+    odt = _DT_OUT.get(out.dtype)
+    if odt is None:
+        raise QIError("out: BF16, FP16 or FP32")
+    if w.get_device() != index or out.get_device() != index:
+        raise QIError("all tensors on one GPU")
+    # a dimension of one element has no stride to go by: any valid one will do
+    (ldx, xc), (ldw, wc), (ldo, oc) = x.stride(), w.stride(), out.stride()
+    if (xc != 1 and K > 1) or (wc != 1 and K > 1) or (oc != 1 and N > 1):
+        raise QIError("rows must be contiguous")
+    if M == 1:
+        ldx, ldo = -(-K // 8) * 8, -(-N // 8) * 8
+    if rows == 1:
+        ldw = -(-K // 8) * 8
+    bp = gp = rp = None
+    ldr = 0
+    if bias is not None:
+        if bias.shape != (rows,) or bias.dtype != xdt or bias.get_device() != index or not bias.is_contiguous():
+            raise QIError("bias: a value for each row of w, in x's type, contiguous, on x's GPU")
+        bp = bias.data_ptr()
+    if gate is not None:
+        if gate.shape != (N,) or gate.dtype != torch.float32 or gate.get_device() != index or not gate.is_contiguous():
+            raise QIError("gate: FP32 [N], contiguous, on x's GPU")
+        gp = gate.data_ptr()
+    if residual is not None:
+        if residual.shape != (M, N) or residual.dtype != out.dtype or residual.get_device() != index:
+            raise QIError("residual: as out")
+        ldr, rc = residual.stride()
+        if rc != 1 and N > 1:
+            raise QIError("rows must be contiguous")
+        if M == 1:
+            ldr = ldo
+        rp = residual.data_ptr()
+    if guard is not None:
+        with guard:
+            return linear_16bit(x, w, bias, act, gate, residual, None, out)
+    st = lib().qi_linear_16bit(x.data_ptr(), ldx, M, K, w.data_ptr(), ldw, N, dt, bp, act, gp, rp, ldr, out.data_ptr(), ldo,
+                               odt, torch._C._cuda_getCurrentRawStream(index))
+    if st:
+        check(st)
     return out
 
 
