@@ -1,75 +1,749 @@
-// prompt_attn.cu -- softmax attention over packed sequences with grouped heads.
+// prompt_attn.cu -- softmax attention over packed sequences with grouped heads,
+// on the 5th-generation tensor cores.
 //
-// One warp per (query, head) walks the keys the query sees with a running
-// maximum m and sum l (FP32, base 2): for score s = scale * log2(e) * q.k,
-//   m' = max(m, s), l' = l 2^(m-m') + 2^(s-m'), o' = o 2^(m-m') + 2^(s-m') v,
-// and out = o / l, or 0 when no key is seen.
+// For one query row with scores s_j = scale log2(e) q.k_j over the keys it sees:
+// running maximum m and sum l (FP32, base 2), weights 2^(s_j - m) rounded to the
+// 16-bit type, O = sum of weights times v in FP32, out = O / l.
+//
+// Work split.  The heads of a group read the same keys, so a 128-row query tile
+// holds T = 128 / P tokens of P heads of one group (P = the group's size up to
+// 128): row = token in tile * P + head.  K and V are read once for the group,
+// and a causal tile spans few positions, so little of its last key block is
+// masked.  A CTA runs NT tiles over one K / V stream; with few tiles the keys
+// are also split over blockIdx.z and a second kernel joins the parts.
+//
+// A CTA's warps: 0 TMA producer, 1 MMA issuer, 2-3 the V guard (below), then a
+// warpgroup of softmax threads per tile (thread = row = TMEM lane).  Per 128-key
+// block and tile: S = Q K^T into TMEM (kind::f16, FP32), the softmax thread reads
+// its row, writes the weights as packed 16-bit over columns 0-63 of S, and
+// O += P V takes P from TMEM and V (token-major) from shared memory.
+//
+// V guard.  A masked weight is 0, but 0 times a NaN or infinity of v is NaN: in
+// blocks with masked keys (the last ones) the guard clears V rows past the
+// sequence's end, and elements that are not finite, before P V reads them, and
+// notes for the latter from which key on they are seen; the epilogue gives
+// exactly the rows that see them the NaN or infinity.
 #include "qi_internal.h"
 #include "sm100.cuh"
+
+#include <limits.h>
+
+#include <type_traits>
 
 namespace qi {
 namespace {
 
-__device__ int g_prompt_attn_err;
+__device__ int g_prompt_attn_err;  // set by a bounded wait that gave up (prompt_attention_take_error)
 
-template <typename T>
-__device__ __forceinline__ float to_f32(T v);
-template <>
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <>
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+constexpr int BQ = 128, BKV = 128;
+constexpr int HALF_BYTES = 128 * 128;  // 128 rows x 64 elements: one swizzled box column
 
-template <typename T>
-__global__ void __launch_bounds__(256) prompt_attn_kernel(const __grid_constant__ PromptAttnArgs a) {
-  const int b = blockIdx.y, h = blockIdx.z, lane = threadIdx.x & 31;
-  const int q0 = min(max(a.q_begin[b], 0), a.total_q), q1 = min(max(a.q_end[b], q0), a.total_q);
-  const int k0 = min(max(a.k_begin[b], 0), a.total_k), k1 = min(max(a.k_end[b], k0), a.total_k);
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= q1 - q0) return;
-  const int seen = a.causal ? min(k1 - k0, max(0, i + 1 + (k1 - k0) - (q1 - q0))) : k1 - k0;
-  const int hk = h / (a.heads / a.kv_heads);
-  const T* q = static_cast<const T*>(a.q) + static_cast<long long>(q0 + i) * a.q_row + h * a.q_head;
-  const T* k = static_cast<const T*>(a.k) + static_cast<long long>(k0) * a.k_row + hk * a.k_head;
-  const T* v = static_cast<const T*>(a.v) + static_cast<long long>(k0) * a.v_row + hk * a.v_head;
-  const float s2 = a.scale * 1.4426950408889634f;
-  float qr[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  for (int e = 0; e < 4; ++e) qr[e] = lane + 32 * e < a.head_dim ? to_f32(q[lane + 32 * e]) : 0.f;
-  for (int j = 0; j < seen; ++j) {
-    float s = 0.f;
-    for (int e = 0; e < 4; ++e)
-      if (lane + 32 * e < a.head_dim) s += qr[e] * to_f32(k[j * a.k_row + lane + 32 * e]);
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    s *= s2;
-    const float mn = fmaxf(m, s), al = m == -INFINITY ? 0.f : exp2f(m - mn), p = exp2f(s - mn);
-    m = mn;
-    l = l * al + p;
-    for (int e = 0; e < 4; ++e)
-      if (lane + 32 * e < a.head_dim) o[e] = o[e] * al + p * to_f32(v[j * a.v_row + lane + 32 * e]);
+template <int DH, int NT>
+struct Cfg {
+  static constexpr int NH = DH / 64;                                // 64-element halves of a head
+  static constexpr int KS = NT == 2 && DH == 128 ? 2 : 3, VS = 2;   // K and V stages
+  static constexpr int THREADS = 128 + 128 * NT;
+  static constexpr int MIN_CTAS = NT == 1 && DH == 64 ? 2 : 1;
+  static constexpr int LAUNCH_REGS = NT == 2 ? 168 : (MIN_CTAS == 2 ? 128 : 256);
+  static constexpr int PRODUCER_REGS = NT == 2 ? 88 : 64, SOFTMAX_REGS = NT == 2 ? 208 : 192;
+  static_assert(128 * PRODUCER_REGS + 128 * NT * SOFTMAX_REGS <= THREADS * LAUNCH_REGS, "register split exceeds the launch");
+  static constexpr int TILE = NH * HALF_BYTES;  // Q tile, K block or V block
+  static constexpr int OFF_K = NT * TILE, OFF_V = OFF_K + KS * TILE, OFF_X = OFF_V + VS * TILE;
+  static constexpr int SMEM = 1024 + OFF_X + 2048;
+  static constexpr int TMEM_COLS = 256 * NT;  // S of tile t at 128 t, O at 128 (NT + t)
+};
+
+struct alignas(64) PromptAttnDev {
+  CUtensorMap tmQ, tmK, tmV;
+  PromptAttnArgs a;
+  int P, T, packs;   // heads per tile row group, tokens per tile, tiles' head packs per kv head
+  int units;         // upper bound of NT-tile units over all sequences (gridDim.x)
+  int chunk, splits;  // key blocks per split; gridDim.z
+  float sc;          // |scale| log2(e)
+  int negate;        // scale < 0: the scores' signs are flipped
+  float* part;       // splits > 1: [splits][total_q * heads][DH] normalised partial outputs
+  float2* ml;        // splits > 1: [splits][total_q * heads] (m, l)
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void settle(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = global_timer_ns();
+  while (!mbar_try_wait(bar, parity) && global_timer_ns() - t0 < kWaitLimitNs / 4) {
   }
-  T* out = static_cast<T*>(a.out) + static_cast<long long>(q0 + i) * a.o_row + h * a.o_head;
-  for (int e = 0; e < 4; ++e)
-    if (lane + 32 * e < a.head_dim) out[lane + 32 * e] = from_f32<T>(seen ? o[e] / l : 0.f);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float a, float b) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack16<__half>(float a, float b) {
+  __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// The sequence that holds unit `u` when every sequence has ceil(Lq / step)
+// units in order, and the unit's index in it; false past the last.  Called by
+// one whole warp.
+struct Place {
+  int seq, unit, q0, lq, k0, lk;
+};
+__device__ __forceinline__ bool clip(const PromptAttnArgs& a, int b, Place& p) {
+  p.q0 = min(max(a.q_begin[b], 0), a.total_q);
+  p.lq = min(max(a.q_end[b], p.q0), a.total_q) - p.q0;
+  p.k0 = min(max(a.k_begin[b], 0), a.total_k);
+  p.lk = min(max(a.k_end[b], p.k0), a.total_k) - p.k0;
+  return true;
+}
+__device__ __forceinline__ bool find_unit(const PromptAttnArgs& a, int step, int u, Place& out) {
+  const int lane = threadIdx.x & 31;
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    Place p = {};
+    int n = 0;
+    if (b0 + lane < a.batch) {
+      clip(a, b0 + lane, p);
+      n = (p.lq + step - 1) / step;
+    }
+    int sum = n;  // inclusive prefix sum over the lanes
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, u < sum);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      out.seq = b0 + src;
+      out.unit = u - __shfl_sync(0xffffffffu, sum - n, src);
+      out.q0 = __shfl_sync(0xffffffffu, p.q0, src);
+      out.lq = __shfl_sync(0xffffffffu, p.lq, src);
+      out.k0 = __shfl_sync(0xffffffffu, p.k0, src);
+      out.lk = __shfl_sync(0xffffffffu, p.lk, src);
+      return true;
+    }
+    u -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return false;
+}
+
+// Last key (relative to the sequence) that token i of the sequence sees, or -1.
+__device__ __forceinline__ int last_seen(int i, int lq, int lk, int causal) {
+  return causal ? max(min(i + lk - lq, lk - 1), -1) : lk - 1;
+}
+
+template <typename T>
+constexpr uint32_t idesc(int M, int N, bool b_mn) {
+  return idesc_f16(M, N, false, b_mn) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u);
+}
+
+template <typename T, int DH, int NT>
+__global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
+    prompt_attn_kernel(const __grid_constant__ PromptAttnDev args) {
+  using C = Cfg<DH, NT>;
+  constexpr int NH = C::NH, KS = C::KS, VS = C::VS, TILE = C::TILE;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sK = smem + C::OFF_K;
+  uint8_t* sV = smem + C::OFF_V;
+  int* bad = reinterpret_cast<int*>(smem + C::OFF_X);  // [3][DH] first key with NaN / +inf / -inf in a dimension
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(bad + 3 * 128);
+  uint64_t* k_full = q_full + 1;       // [KS]
+  uint64_t* k_empty = k_full + KS;     // [KS]
+  uint64_t* v_full = k_empty + KS;     // [VS]
+  uint64_t* v_ready = v_full + VS;     // [VS] the V guard has passed the block (2 warps)
+  uint64_t* v_empty = v_ready + VS;    // [VS]
+  uint64_t* s_full = v_empty + VS;     // [NT] QK of the tile's current block complete
+  uint64_t* s_loaded = s_full + NT;    // [NT] the tile's S is in registers (4 warps)
+  uint64_t* p_half = s_loaded + NT;    // [NT][2] half h of the tile's P is in TMEM (4 warps)
+  uint64_t* o_final = p_half + 2 * NT; // [NT] the tile's last PV complete
+  uint64_t* drain = o_final + NT;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* any_bad = const_cast<int*>(abort_flag) + 1;
+  Place* place = reinterpret_cast<Place*>(any_bad + 1);
+  int* found = reinterpret_cast<int*>(place + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PromptAttnArgs& a = args.a;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < KS; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < VS; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_ready[i], 2);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int t = 0; t < NT; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&s_loaded[t], 4);
+      mbar_init(&p_half[2 * t], 4);
+      mbar_init(&p_half[2 * t + 1], 4);
+      mbar_init(&o_final[t], 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    *any_bad = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&args.tmQ);
+    tma_prefetch_desc(&args.tmK);
+    tma_prefetch_desc(&args.tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  if (warp == 2)
+    for (int i = lane; i < 3 * DH; i += 32) bad[i] = INT_MAX;
+  grid_dependency_wait();
+  launch_dependents();
+  if (warp == 0) {  // units in descending order: a causal sequence's later units have more keys
+    Place p;
+    const bool ok = find_unit(a, NT * args.T, args.units - 1 - static_cast<int>(blockIdx.x), p);
+    if (lane == 0) {
+      *place = p;
+      *found = ok;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const Place pl = *place;
+  const int tok0 = pl.unit * NT * args.T;  // first token of the unit in its sequence
+  // key blocks [jb, je[t]) of tile t in this split; n[t] of them
+  int n[NT], nkb[NT], nmax = 0;
+  const int jb = static_cast<int>(blockIdx.z) * args.chunk;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int first = tok0 + t * args.T, lim = last_seen(min(first + args.T, pl.lq) - 1, pl.lq, pl.lk, a.causal);
+    nkb[t] = *found && first < pl.lq ? (lim + BKV) / BKV : 0;  // lim = -1: none
+    const int je = static_cast<int>(blockIdx.z) == args.splits - 1 ? nkb[t] : min(nkb[t], jb + args.chunk);
+    n[t] = max(0, je - jb);
+    nmax = max(nmax, n[t]);
+  }
+  // keys past the first token's last are masked for some row
+  const int lim_first = last_seen(tok0, pl.lq, pl.lk, a.causal);
+  const int y = blockIdx.y, hk = y / args.packs;
+
+  if (warp < 4) {
+    if (C::LAUNCH_REGS < 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::PRODUCER_REGS));
+    if (warp == 0) {
+      // -------------------------------------------------------------- producer
+      if (lane == 0 && nmax > 0) {
+        bool ok = true;
+        uint32_t kmask = 0, kpar = 0, vmask = 0, vpar = 0;
+        mbar_expect_tx(q_full, NT * NH * args.T * args.P * 128);
+        for (int t = 0; t < NT; ++t)
+          for (int h = 0; h < NH; ++h)
+            tma_load_4d(sQ + t * TILE + h * HALF_BYTES, &args.tmQ, 64 * h, 0, pl.q0 + tok0 + t * args.T, y, q_full);
+        for (int i = 0; i < nmax && ok; ++i) {
+          const int ks = i % KS, vs = i % VS, row = pl.k0 + (jb + i) * BKV;
+          const uint32_t kp = (i / KS) & 1, vp = (i / VS) & 1;
+          if (!mbar_wait(&k_empty[ks], kp ^ 1u, abort_flag)) { ok = false; break; }
+          mbar_expect_tx(&k_full[ks], TILE);
+          for (int h = 0; h < NH; ++h) tma_load_3d(sK + ks * TILE + h * HALF_BYTES, &args.tmK, 64 * h, hk, row, &k_full[ks]);
+          kmask |= 1u << ks;
+          kpar = (kpar & ~(1u << ks)) | (kp << ks);
+          if (!mbar_wait(&v_empty[vs], vp ^ 1u, abort_flag)) { ok = false; break; }
+          mbar_expect_tx(&v_full[vs], TILE);
+          for (int h = 0; h < NH; ++h) tma_load_3d(sV + vs * TILE + h * HALF_BYTES, &args.tmV, 64 * h, hk, row, &v_full[vs]);
+          vmask |= 1u << vs;
+          vpar = (vpar & ~(1u << vs)) | (vp << vs);
+        }
+        if (!ok) {  // let the copies already issued land before the CTA exits
+          *abort_flag = 1;
+          atomicCAS(&g_prompt_attn_err, 0, kErrTimeoutProducer);
+          settle(q_full, 0);
+          for (int s = 0; s < KS; ++s)
+            if (kmask & (1u << s)) settle(&k_full[s], (kpar >> s) & 1u);
+          for (int s = 0; s < VS; ++s)
+            if (vmask & (1u << s)) settle(&v_full[s], (vpar >> s) & 1u);
+        }
+      }
+    } else if (warp == 1) {
+      // -------------------------------------------------------------- MMA issuer
+      if (nmax > 0) {
+        // every lane waits; the vote keeps the warp converged for elect.sync
+        auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+          return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+        };
+        const uint32_t id_qk = idesc<T>(BQ, BKV, false), id_qk64 = idesc<T>(BQ, 64, false), id_pv = idesc<T>(BQ, DH, true);
+        const uint64_t qd0 = umma_desc_sw128(smem_u32(sQ), 16, 1024), kd0 = umma_desc_sw128(smem_u32(sK), 16, 1024);
+        const uint64_t vd0 = umma_desc_sw128(smem_u32(sV), HALF_BYTES, 1024);
+        // S_t = Q_t K^T: all 128 keys, or keys 64 hh .. of them (columns 64 hh ..)
+        auto qk = [&](int t, int ks) {
+#pragma unroll
+          for (int k = 0; k < DH / 16; ++k) {
+            const uint64_t off = (k / 4) * (HALF_BYTES >> 4) + 2 * (k % 4);
+            mma_f16_ss_elect(tmem + 128 * t, qd0 + static_cast<uint64_t>((t * TILE) >> 4) + off,
+                             kd0 + static_cast<uint64_t>((ks * TILE) >> 4) + off, id_qk, k > 0 ? 1u : 0u);
+          }
+        };
+        auto qk_half = [&](int t, int ks, int hh) {
+#pragma unroll
+          for (int k = 0; k < DH / 16; ++k) {
+            const uint64_t off = (k / 4) * (HALF_BYTES >> 4) + 2 * (k % 4);
+            mma_f16_ss_elect(tmem + 128 * t + 64 * hh, qd0 + static_cast<uint64_t>((t * TILE) >> 4) + off,
+                             kd0 + static_cast<uint64_t>((ks * TILE + hh * (HALF_BYTES / 2)) >> 4) + off, id_qk64,
+                             k > 0 ? 1u : 0u);
+          }
+        };
+        // O_t += P_t V over keys 64 h .. of the block
+        auto pv_half = [&](int t, int vs, int i, int h) {
+#pragma unroll
+          for (int k4 = 0; k4 < 4; ++k4) {
+            const int kk = 4 * h + k4;
+            mma_f16_ts_elect(tmem + 128 * (NT + t), tmem + 128 * t + 8 * kk,
+                             vd0 + static_cast<uint64_t>((vs * TILE) >> 4) + 128 * kk, id_pv, (i > 0 || kk > 0) ? 1u : 0u);
+          }
+        };
+        bool ok = wait_all(q_full, 0) && wait_all(&k_full[0], 0);
+        if (ok) {
+          tc_fence_after();
+          for (int t = 0; t < NT; ++t) {
+            if (n[t] == 0) continue;
+            qk(t, 0);
+            mma_commit_elect(&s_full[t]);
+          }
+          mma_commit_elect(&k_empty[0]);
+        }
+        for (int i = 0; i < nmax && ok; ++i) {
+          const int vs = i % VS, ks = (i + 1) % KS;
+          const uint32_t vp = (i / VS) & 1, kp = ((i + 1) / KS) & 1;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if (!ok || i >= n[t]) continue;
+            const bool more = i + 1 < n[t];
+            // the last tile that still uses this V block / the next K block
+            const bool last_v = t == NT - 1 || i >= n[NT - 1], last_k = t == NT - 1 || i + 1 >= n[NT - 1];
+            if (more) {  // upper half of S_t for the next block: its columns never hold P
+              ok = wait_all(&s_loaded[t], i & 1) && wait_all(&k_full[ks], kp);
+              if (!ok) break;
+              tc_fence_after();
+              qk_half(t, ks, 1);
+            }
+            ok = wait_all(&p_half[2 * t], i & 1) && wait_all(&v_ready[vs], vp);
+            if (!ok) break;
+            tc_fence_after();
+            pv_half(t, vs, i, 0);
+            ok = wait_all(&p_half[2 * t + 1], i & 1);
+            if (!ok) break;
+            tc_fence_after();
+            pv_half(t, vs, i, 1);
+            if (!more) mma_commit_elect(&o_final[t]);
+            if (last_v) mma_commit_elect(&v_empty[vs]);
+            if (more) {
+              // the lower half overwrites the columns P_t V reads: it is issued
+              // behind it, and a CTA's MMAs run in issue order
+              qk_half(t, ks, 0);
+              mma_commit_elect(&s_full[t]);
+              if (last_k) mma_commit_elect(&k_empty[ks]);
+            }
+          }
+        }
+        if (!ok && lane == 0) {
+          *abort_flag = 1;
+          atomicCAS(&g_prompt_attn_err, 0, kErrTimeoutMma);
+        }
+        __syncwarp();
+        mma_commit_elect(drain);  // every MMA issued above completes before TMEM is released
+        settle(drain, 0);
+      }
+    } else {
+      // -------------------------------------------------------------- V guard
+      constexpr uint32_t EXP = std::is_same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;  // NaN or infinity: all set
+      bool ok = true;
+      for (int i = 0; i < nmax && ok; ++i) {
+        const int vs = i % VS, key0 = (jb + i) * BKV;
+        ok = __all_sync(0xffffffffu, mbar_wait(&v_full[vs], (i / VS) & 1, abort_flag));
+        if (!ok) break;
+        if (key0 + BKV - 1 > lim_first) {
+#pragma unroll 4
+          for (int c = (warp - 2) * 32 + lane; c < NH * 1024; c += 64) {
+            const int half = c >> 10, r = (c >> 3) & 127, pc = c & 7;
+            if (key0 + r <= lim_first) continue;
+            uint4* p = reinterpret_cast<uint4*>(sV + vs * TILE + half * HALF_BYTES + r * 128 + pc * 16);
+            if (key0 + r >= pl.lk) {
+              *p = make_uint4(0u, 0u, 0u, 0u);
+              continue;
+            }
+            const uint4 v = *p;
+            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              any |= ((u[e] & EXP) == EXP) | ((u[e] & (EXP << 16)) == (EXP << 16));
+            if (any) {
+              uint16_t* q = reinterpret_cast<uint16_t*>(p);
+              for (int e = 0; e < 8; ++e) {
+                const uint32_t w = q[e];
+                if ((w & EXP) != EXP) continue;
+                const int kind = (w & (0x7FFFu ^ EXP)) ? 0 : (w & 0x8000u ? 2 : 1);
+                atomicMin(&bad[kind * DH + half * 64 + (pc ^ (r & 7)) * 8 + e], key0 + r);
+                q[e] = 0;
+                *any_bad = 1;
+              }
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_ready[vs]);
+      }
+      if (!ok && lane == 0) {
+        *abort_flag = 1;
+        atomicCAS(&g_prompt_attn_err, 0, kErrTimeoutSoftmax);
+      }
+    }
+  } else {
+    if (C::LAUNCH_REGS < 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
+    // ---------------------------------------------------------------- softmax
+    const int t = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const int my_n = NT == 1 || t == 0 ? n[0] : n[NT - 1], my_nkb = NT == 1 || t == 0 ? nkb[0] : nkb[NT - 1];
+    const int tok = row / args.P, i_tok = tok0 + t * args.T + tok;  // token in its sequence
+    const bool valid = *found && tok < args.T && i_tok < pl.lq;
+    const int lim = valid ? last_seen(i_tok, pl.lq, pl.lk, a.causal) : -1;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_tm = tmem + lane_off + 128 * t, o_tm = tmem + lane_off + 128 * (NT + t);
+    // FP16 weights are kept in 2^7 .. 2^15 for the largest so that small ones
+    // stay clear of the subnormals; the factor is in l too
+    constexpr float LIFT = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+    const uint64_t sc2 = f2pack(args.sc, args.sc);
+    const uint32_t flip = args.negate ? 0x80000000u : 0u;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int i = 0; i < my_n; ++i) {
+      const bool w = mbar_wait(&s_full[t], i & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, w)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t r[BKV];
+#pragma unroll
+      for (int c = 0; c < BKV; c += 32) tmem_ld32(s_tm + c, *reinterpret_cast<uint32_t(*)[32]>(r + c));
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < BKV; c += 32) tmem_reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(r + c));
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_loaded[t]);
+      const int key0 = (jb + i) * BKV, seen = lim - key0;  // keys 0 .. seen of the block are seen
+      if (flip) {
+#pragma unroll
+        for (int c = 0; c < BKV; ++c) r[c] ^= flip;
+      }
+      const bool masked = __any_sync(0xffffffffu, seen < BKV - 1);
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < BKV; ++c)
+          if (c > seen) r[c] = 0xFF800000u;  // -inf
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < BKV; c += 4)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(r[c + e]));
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      // Lazy rescale: the maximum used moves only when the row's grows by more
+      // than 8 (weights stay <= 2^8); O and l move with it
+      const float m_new = fmaxf(m, top == -INFINITY ? -INFINITY : top * args.sc);
+      const bool grow = m_new > m + 8.0f;
+      const float alpha = grow ? ex2(m - m_new) : 1.0f;
+      if (grow) m = m_new;
+      if (i > 0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll 1
+        for (int c = 0; c < DH; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_tm + c, o);
+          tmem_ld_wait();
+          tmem_reg_fence32(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st32(o_tm + c, o);
+        }
+      }
+      const float base = m == -INFINITY ? 0.0f : LIFT - m;  // nothing seen yet: every weight is 0
+      const uint64_t base2 = f2pack(base, base);
+      uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const int k = 64 * h + 2 * c;
+          float p0, p1;
+          f2unpack(f2fma(f2pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), sc2, base2), p0, p1);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          if (masked) {
+            if (k > seen) p0 = 0.0f;
+            if (k + 1 > seen) p1 = 0.0f;
+          }
+          sum2[c & 3] = f2add(sum2[c & 3], f2pack(p0, p1));
+          pk[c] = pack16<T>(p0, p1);
+        }
+        tmem_st32(s_tm + 32 * h, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_half[2 * t + h]);
+      }
+      float a0, a1;
+      f2unpack(f2add(f2add(sum2[0], sum2[1]), f2add(sum2[2], sum2[3])), a0, a1);
+      l = l * alpha + (a0 + a1);
+    }
+    if (ok && my_n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_final[t], 0, abort_flag));
+    if (!ok) {
+      if (lane == 0) {
+        *abort_flag = 1;
+        atomicCAS(&g_prompt_attn_err, 0, kErrTimeoutSoftmax);
+      }
+    } else {
+      // ---------------------------------------------------------------- epilogue
+      tc_fence_after();
+      // splits of this tile that hold keys; with one the output is final
+      const int used = min(args.splits, max(1, (my_nkb + args.chunk - 1) / args.chunk));
+      const bool mine = valid && static_cast<int>(blockIdx.z) < used;
+      const float rl = l == 0.0f ? 0.0f : 1.0f / l;  // NaN stays NaN
+      const int head = y * args.P + row % args.P;
+      const long long qrow = pl.q0 + i_tok, slot = qrow * a.heads + head;
+      T* out = static_cast<T*>(a.out) + qrow * a.o_row + head * a.o_head;
+      const long long part_rows = static_cast<long long>(a.total_q) * a.heads;
+      float* part = args.part + (static_cast<long long>(blockIdx.z) * part_rows + slot) * DH;
+      const bool patch = *any_bad != 0;
+#pragma unroll 1
+      for (int c = 0; c < DH; c += 32) {
+        uint32_t o[32];
+        __syncwarp();
+        if (my_n > 0) {
+          tmem_ld32(o_tm + c, o);
+          tmem_ld_wait();
+          tmem_reg_fence32(o);
+        }
+        if (!mine) continue;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[e]) * rl);
+        if (patch && l != 0.0f) {
+          for (int e = 0; e < 32; ++e) {
+            const bool nan = bad[c + e] <= lim, pos = bad[DH + c + e] <= lim, neg = bad[2 * DH + c + e] <= lim;
+            if (nan | (pos & neg)) o[e] = 0x7FFFFFFFu;
+            else if (pos | neg) o[e] = __float_as_uint(__uint_as_float(o[e]) + (pos ? INFINITY : -INFINITY));
+          }
+        }
+        if (used > 1) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<uint4*>(part + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8)
+            if (c + e < a.head_dim)
+              *reinterpret_cast<uint4*>(out + c + e) =
+                  make_uint4(pack16<T>(__uint_as_float(o[e]), __uint_as_float(o[e + 1])),
+                             pack16<T>(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])),
+                             pack16<T>(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5])),
+                             pack16<T>(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])));
+        }
+      }
+      if (mine && used > 1) args.ml[static_cast<long long>(blockIdx.z) * part_rows + slot] = make_float2(m, l);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+// Joins the splits of a row: out = sum_s w_s O_s / sum_s w_s, w_s = l_s 2^(m_s - max m).
+// One warp per (token, head), four dimensions per thread; rows whose tile had
+// one split are final already.
+template <typename T, int DH>
+__global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_constant__ PromptAttnDev args) {
+  grid_dependency_wait();
+  launch_dependents();
+  const PromptAttnArgs& a = args.a;
+  const int lane = threadIdx.x & 31;
+  const long long slot = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const long long rows = static_cast<long long>(a.total_q) * a.heads;
+  if (slot >= rows) return;
+  const int qrow = static_cast<int>(slot / a.heads), head = static_cast<int>(slot % a.heads);
+  Place p = {};
+  bool found = false;
+  for (int b0 = 0; b0 < a.batch && !found; b0 += 32) {
+    Place c = {};
+    bool hit = false;
+    if (b0 + lane < a.batch) {
+      clip(a, b0 + lane, c);
+      hit = qrow >= c.q0 && qrow < c.q0 + c.lq;
+    }
+    const unsigned m = __ballot_sync(0xffffffffu, hit);
+    if (m) {
+      found = true;
+      const int src = __ffs(m) - 1;
+      p.q0 = __shfl_sync(0xffffffffu, c.q0, src);
+      p.lq = __shfl_sync(0xffffffffu, c.lq, src);
+      p.lk = __shfl_sync(0xffffffffu, c.lk, src);
+    }
+  }
+  if (!found) return;
+  const int tile_end = min(((qrow - p.q0) / args.T + 1) * args.T, p.lq) - 1;
+  const int nkb = (last_seen(tile_end, p.lq, p.lk, a.causal) + BKV) / BKV;
+  const int used = min(args.splits, max(1, (nkb + args.chunk - 1) / args.chunk));
+  if (used <= 1 || 4 * lane >= DH) return;
+  float top = -INFINITY;
+  for (int s = 0; s < used; ++s) top = fmaxf(top, args.ml[s * rows + slot].x);
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float total = 0.0f;
+  for (int s = 0; s < used; ++s) {
+    const float2 ml = args.ml[s * rows + slot];
+    if (ml.y == 0.0f) continue;  // this part saw nothing
+    const float w = ml.y * ex2(ml.x - top);
+    const float4 v = *reinterpret_cast<const float4*>(args.part + (s * rows + slot) * DH + 4 * lane);
+    total += w;
+    o = make_float4(o.x + w * v.x, o.y + w * v.y, o.z + w * v.z, o.w + w * v.w);
+  }
+  const float r = total == 0.0f ? 0.0f : 1.0f / total;
+  if (4 * lane >= a.head_dim) return;
+  T* out = static_cast<T*>(a.out) + qrow * a.o_row + head * a.o_head + 4 * lane;
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(o.x * r, o.y * r), pack16<T>(o.z * r, o.w * r));
+}
+
+// ------------------------------------------------------------------ host
+struct Plan {
+  int P, T, packs, nt, chunk, splits, dh;
+  long long units;
+};
+
+Plan plan_of(int heads, int kv_heads, int head_dim, int batch, int total_q, int max_k, int num_sms) {
+  Plan p;
+  const int G = heads / kv_heads;
+  p.dh = head_dim <= 64 ? 64 : 128;
+  p.P = G;
+  while (p.P > BQ || G % p.P) --p.P;
+  p.T = BQ / p.P;
+  p.packs = G / p.P;
+  const long long ctas1 = (static_cast<long long>(total_q) / p.T + batch) * (heads / p.P);
+  // one tile per CTA while those fit on the device at once (shorter calls), two
+  // over one K / V stream beyond that
+  p.nt = ctas1 <= num_sms ? 1 : 2;
+  p.units = static_cast<long long>(total_q) / (p.nt * p.T) + batch;
+  const long long ctas = p.units * (heads / p.P);
+  const int blocks = max_k / BKV + (max_k % BKV != 0);
+  // key splits: fill the device (two CTAs per SM with heads of 64)
+  const long long slots = static_cast<long long>(num_sms) * (p.nt == 1 && p.dh == 64 ? 2 : 1);
+  long long splits = ctas < slots ? slots / ctas : 1;
+  if (splits > (blocks + 1) / 2) splits = (blocks + 1) / 2;  // two blocks each at least
+  if (splits < 1) splits = 1;
+  p.chunk = blocks > 0 ? static_cast<int>((blocks + splits - 1) / splits) : 1;
+  p.splits = blocks > 0 ? (blocks + p.chunk - 1) / p.chunk : 1;
+  return p;
+}
+
+int encode_heads(CUtensorMap* tm, int dtype, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                 const cuuint32_t* box) {
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = qi_encode_tiled(tm, dtype == QI_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                                     rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? QI_OK : QI_ERR_CUDA;
+}
+
+template <typename A>
+int launch_dependent(void (*fn)(const A), dim3 grid, int threads, int smem, const A& args, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fn, args) == cudaSuccess ? QI_OK : QI_ERR_CUDA;
+}
+
+template <typename T, int DH, int NT>
+int launch_tiles(const PromptAttnDev& d, cudaStream_t stream) {
+  using C = Cfg<DH, NT>;
+  static_assert(C::SMEM <= 227 * 1024, "shared memory");
+  static unsigned long long attr_done = 0;
+  const auto fn = prompt_attn_kernel<T, DH, NT>;
+  if (smem_optin(reinterpret_cast<const void*>(fn), C::SMEM, &attr_done) != QI_OK) return QI_ERR_CUDA;
+  const dim3 grid(d.units, d.a.heads / d.P, d.splits);
+  const int st = launch_dependent(fn, grid, C::THREADS, C::SMEM, d, stream);
+  if (st != QI_OK || d.splits == 1) return st;
+  const long long rows = static_cast<long long>(d.a.total_q) * d.a.heads;
+  return launch_dependent(prompt_attn_join_kernel<T, DH>, dim3(static_cast<unsigned>((rows + 7) / 8)), 256, 0, d, stream);
+}
+
+template <typename T>
+int launch_typed(const PromptAttnDev& d, int nt, int dh, cudaStream_t stream) {
+  if (dh == 64) return nt == 1 ? launch_tiles<T, 64, 1>(d, stream) : launch_tiles<T, 64, 2>(d, stream);
+  return nt == 1 ? launch_tiles<T, 128, 1>(d, stream) : launch_tiles<T, 128, 2>(d, stream);
 }
 
 }  // namespace
 
 long long prompt_attention_workspace(int heads, int kv_heads, int head_dim, int batch, int total_q, int max_k) {
-  return 0;
+  if (batch == 0 || total_q == 0) return 0;
+  const Plan p = plan_of(heads, kv_heads, head_dim, batch, total_q, max_k, device_num_sms());
+  if (p.splits == 1) return 0;
+  return static_cast<long long>(p.splits) * total_q * heads * (p.dh * 4 + 8);
 }
 
 int prompt_attention_launch(const PromptAttnArgs& a, cudaStream_t stream) {
-  const dim3 grid((a.total_q + 7) / 8, a.batch, a.heads);
-  if (a.dtype == QI_DT_BF16)
-    prompt_attn_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a);
-  else
-    prompt_attn_kernel<__half><<<grid, 256, 0, stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? QI_OK : QI_ERR_CUDA;
+  const Plan p = plan_of(a.heads, a.kv_heads, a.head_dim, a.batch, a.total_q, a.max_k, device_num_sms());
+  if (p.units > 0x7fffffffll) return QI_ERR_UNSUPPORTED;
+  PromptAttnDev d;
+  memset(&d, 0, sizeof(d));
+  d.a = a;
+  d.P = p.P;
+  d.T = p.T;
+  d.packs = p.packs;
+  d.units = static_cast<int>(p.units);
+  d.chunk = p.chunk;
+  d.splits = p.splits;
+  d.sc = (a.scale < 0.0f ? -a.scale : a.scale) * 1.4426950408889634f;
+  d.negate = a.scale < 0.0f;
+  if (p.splits > 1) {
+    const long long rows = static_cast<long long>(a.total_q) * a.heads;
+    d.part = static_cast<float*>(a.workspace);
+    d.ml = reinterpret_cast<float2*>(d.part + p.splits * rows * p.dh);
+  }
+  // a dimension of one element has no stride to go by: any valid one will do
+  auto stride = [](long long s, long long n) { return static_cast<cuuint64_t>(n > 1 ? s * 2 : 16); };
+  const cuuint64_t dim = a.head_dim;
+  {  // Q: (d, head of the pack, token, pack): a tile's rows are token-major, heads inside
+    cuuint64_t dims[4] = {dim, static_cast<cuuint64_t>(p.P), static_cast<cuuint64_t>(a.total_q),
+                          static_cast<cuuint64_t>(a.heads / p.P)};
+    cuuint64_t str[3] = {stride(a.q_head, p.P), stride(a.q_row, a.total_q), stride(a.q_head * p.P, a.heads / p.P)};
+    cuuint32_t box[4] = {64, static_cast<cuuint32_t>(p.P), static_cast<cuuint32_t>(p.T), 1};
+    if (encode_heads(&d.tmQ, a.dtype, a.q, 4, dims, str, box) != QI_OK) return QI_ERR_CUDA;
+  }
+  // K, V: (d, kv head, row); without rows the base is never read, and any will do
+  auto kv = [&](CUtensorMap* tm, const void* base, long long row, long long head) {
+    cuuint64_t dims[3] = {dim, static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.total_k > 0 ? a.total_k : 1)};
+    cuuint64_t str[2] = {stride(head, a.kv_heads), stride(row, a.total_k)};
+    cuuint32_t box[3] = {64, 1, BKV};
+    return encode_heads(tm, a.dtype, a.total_k > 0 ? base : a.q, 3, dims, str, box);
+  };
+  if (kv(&d.tmK, a.k, a.k_row, a.k_head) != QI_OK || kv(&d.tmV, a.v, a.v_row, a.v_head) != QI_OK) return QI_ERR_CUDA;
+  return a.dtype == QI_DT_BF16 ? launch_typed<__nv_bfloat16>(d, p.nt, p.dh, stream)
+                               : launch_typed<__half>(d, p.nt, p.dh, stream);
 }
 
 int prompt_attention_take_error(int* bad) {

@@ -31,7 +31,7 @@ int check_stride(long long stride, long long n) {
 int check_sizes(int heads, int kv_heads, int head_dim, int batch, int total_q, int total_k, int max_k) {
   if (heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1) return QI_ERR_ARG;
   if (batch < 0 || total_q < 0 || total_k < 0 || max_k < 0) return QI_ERR_ARG;
-  if (head_dim % 8 || head_dim > 128 || kv_heads > 65535) return QI_ERR_UNSUPPORTED;
+  if (head_dim % 8 || head_dim > 128 || heads > 65535) return QI_ERR_UNSUPPORTED;
   return QI_OK;
 }
 }  // namespace
