@@ -19,10 +19,10 @@
 // O += P V takes P from TMEM and V (token-major) from shared memory.
 //
 // V guard.  A masked weight is 0, but 0 times a NaN or infinity of v is NaN: in
-// blocks with masked keys (the last ones) the guard clears V rows past the
-// sequence's end, and elements that are not finite, before P V reads them, and
-// notes for the latter from which key on they are seen; the epilogue gives
-// exactly the rows that see them the NaN or infinity.
+// blocks with masked keys (the last ones) the guard clears the V rows that no
+// row of the CTA sees and, in rows that only some see, the elements that are not
+// finite, before P V reads them.  It notes from which key on those are seen, and
+// the epilogue gives exactly the rows that see them the NaN or infinity.
 #include "qi_internal.h"
 #include "sm100.cuh"
 
@@ -54,13 +54,13 @@ struct Cfg {
 };
 
 struct alignas(64) PromptAttnDev {
-  CUtensorMap tmQ, tmK, tmV;
+  CUtensorMap tmQ, tmK, tmV, tmO;
   PromptAttnArgs a;
   int P, T, packs;   // heads per tile row group, tokens per tile, tiles' head packs per kv head
   int units;         // upper bound of NT-tile units over all sequences (gridDim.x)
   int chunk, splits;  // key blocks per split; gridDim.z
   float sc;          // |scale| log2(e)
-  int negate;        // scale < 0: the scores' signs are flipped
+  uint32_t negate;   // scale < 0: instruction descriptor bit 13 (negate A) for Q K^T
   float* part;       // splits > 1: [splits][total_q * heads][DH] normalised partial outputs
   float2* ml;        // splits > 1: [splits][total_q * heads] (m, l)
 };
@@ -68,6 +68,11 @@ struct alignas(64) PromptAttnDev {
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 __device__ __forceinline__ void settle(uint64_t* bar, uint32_t parity) {
@@ -232,8 +237,10 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
     n[t] = max(0, je - jb);
     nmax = max(nmax, n[t]);
   }
-  // keys past the first token's last are masked for some row
+  // keys past the first token's last are masked for some row, past the unit's
+  // last token's for all
   const int lim_first = last_seen(tok0, pl.lq, pl.lk, a.causal);
+  const int lim_unit = last_seen(min(tok0 + NT * args.T, pl.lq) - 1, pl.lq, pl.lk, a.causal);
   const int y = blockIdx.y, hk = y / args.packs;
 
   if (warp < 4) {
@@ -278,7 +285,8 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
         auto wait_all = [&](uint64_t* bar, uint32_t parity) {
           return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
         };
-        const uint32_t id_qk = idesc<T>(BQ, BKV, false), id_qk64 = idesc<T>(BQ, 64, false), id_pv = idesc<T>(BQ, DH, true);
+        const uint32_t id_qk = idesc<T>(BQ, BKV, false) | args.negate, id_qk64 = idesc<T>(BQ, 64, false) | args.negate;
+        const uint32_t id_pv = idesc<T>(BQ, DH, true);
         const uint64_t qd0 = umma_desc_sw128(smem_u32(sQ), 16, 1024), kd0 = umma_desc_sw128(smem_u32(sK), 16, 1024);
         const uint64_t vd0 = umma_desc_sw128(smem_u32(sV), HALF_BYTES, 1024);
         // S_t = Q_t K^T: all 128 keys, or keys 64 hh .. of them (columns 64 hh ..)
@@ -369,33 +377,35 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
         ok = __all_sync(0xffffffffu, mbar_wait(&v_full[vs], (i / VS) & 1, abort_flag));
         if (!ok) break;
         if (key0 + BKV - 1 > lim_first) {
-#pragma unroll 4
-          for (int c = (warp - 2) * 32 + lane; c < NH * 1024; c += 64) {
-            const int half = c >> 10, r = (c >> 3) & 127, pc = c & 7;
-            if (key0 + r <= lim_first) continue;
-            uint4* p = reinterpret_cast<uint4*>(sV + vs * TILE + half * HALF_BYTES + r * 128 + pc * 16);
-            if (key0 + r >= pl.lk) {
-              *p = make_uint4(0u, 0u, 0u, 0u);
-              continue;
-            }
-            const uint4 v = *p;
-            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-            bool any = false;
+          // 16-byte pieces of the rows nobody sees (cleared), and before them of
+          // the rows that some see and some do not (checked)
+          const int scan0 = max(lim_first + 1 - key0, 0) * 8, zero0 = min(max(lim_unit + 1 - key0, 0), BKV) * 8;
+          uint8_t* blk = sV + vs * TILE;
+          for (int c = zero0 + (warp - 2) * 32 + lane; c < BKV * 8; c += 64)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              any |= ((u[e] & EXP) == EXP) | ((u[e] & (EXP << 16)) == (EXP << 16));
-            if (any) {
-              uint16_t* q = reinterpret_cast<uint16_t*>(p);
-              for (int e = 0; e < 8; ++e) {
-                const uint32_t w = q[e];
-                if ((w & EXP) != EXP) continue;
-                const int kind = (w & (0x7FFFu ^ EXP)) ? 0 : (w & 0x8000u ? 2 : 1);
-                atomicMin(&bad[kind * DH + half * 64 + (pc ^ (r & 7)) * 8 + e], key0 + r);
-                q[e] = 0;
-                *any_bad = 1;
+            for (int h = 0; h < NH; ++h) *reinterpret_cast<uint4*>(blk + h * HALF_BYTES + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+          for (int c = scan0 + (warp - 2) * 32 + lane; c < zero0; c += 64)
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+              uint8_t* p = blk + h * HALF_BYTES + c * 16;
+              const uint4 v = *reinterpret_cast<const uint4*>(p);
+              const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+              bool any = false;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                any |= ((u[e] & EXP) == EXP) | ((u[e] & (EXP << 16)) == (EXP << 16));
+              if (any) {
+                uint16_t* q = reinterpret_cast<uint16_t*>(p);
+                for (int e = 0; e < 8; ++e) {
+                  const uint32_t w = q[e];
+                  if ((w & EXP) != EXP) continue;
+                  const int kind = (w & (0x7FFFu ^ EXP)) ? 0 : (w & 0x8000u ? 2 : 1);
+                  atomicMin(&bad[kind * DH + h * 64 + ((c & 7) ^ ((c >> 3) & 7)) * 8 + e], key0 + (c >> 3));
+                  q[e] = 0;
+                  *any_bad = 1;
+                }
               }
             }
-          }
           fence_proxy_async_smem();
         }
         __syncwarp();
@@ -420,7 +430,6 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
     // stay clear of the subnormals; the factor is in l too
     constexpr float LIFT = std::is_same<T, __half>::value ? 7.0f : 0.0f;
     const uint64_t sc2 = f2pack(args.sc, args.sc);
-    const uint32_t flip = args.negate ? 0x80000000u : 0u;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     for (int i = 0; i < my_n; ++i) {
@@ -437,121 +446,179 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
       __syncwarp();
       if (lane == 0) mbar_arrive(&s_loaded[t]);
       const int key0 = (jb + i) * BKV, seen = lim - key0;  // keys 0 .. seen of the block are seen
-      if (flip) {
-#pragma unroll
-        for (int c = 0; c < BKV; ++c) r[c] ^= flip;
-      }
-      const bool masked = __any_sync(0xffffffffu, seen < BKV - 1);
-      if (masked) {
-#pragma unroll
-        for (int c = 0; c < BKV; ++c)
-          if (c > seen) r[c] = 0xFF800000u;  // -inf
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < BKV; c += 4)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(r[c + e]));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      // Lazy rescale: the maximum used moves only when the row's grows by more
-      // than 8 (weights stay <= 2^8); O and l move with it
-      const float m_new = fmaxf(m, top == -INFINITY ? -INFINITY : top * args.sc);
-      const bool grow = m_new > m + 8.0f;
-      const float alpha = grow ? ex2(m - m_new) : 1.0f;
-      if (grow) m = m_new;
-      if (i > 0 && __any_sync(0xffffffffu, grow)) {
-#pragma unroll 1
-        for (int c = 0; c < DH; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(o_tm + c, o);
-          tmem_ld_wait();
-          tmem_reg_fence32(o);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tmem_st32(o_tm + c, o);
-        }
-      }
-      const float base = m == -INFINITY ? 0.0f : LIFT - m;  // nothing seen yet: every weight is 0
-      const uint64_t base2 = f2pack(base, base);
+      float alpha = 1.0f;
       uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
+      auto block = [&](auto masked_tag) {
+        constexpr bool MASKED = decltype(masked_tag)::value;
+        if (MASKED) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const int k = 64 * h + 2 * c;
-          float p0, p1;
-          f2unpack(f2fma(f2pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), sc2, base2), p0, p1);
-          p0 = ex2(p0);
-          p1 = ex2(p1);
-          if (masked) {
-            if (k > seen) p0 = 0.0f;
-            if (k + 1 > seen) p1 = 0.0f;
-          }
-          sum2[c & 3] = f2add(sum2[c & 3], f2pack(p0, p1));
-          pk[c] = pack16<T>(p0, p1);
+          for (int c = 0; c < BKV; ++c)
+            if (c > seen) r[c] = 0xFF800000u;  // -inf
         }
-        tmem_st32(s_tm + 32 * h, pk);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_half[2 * t + h]);
-      }
+        float mx[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(r[e]);
+#pragma unroll
+        for (int c = 4; c < BKV - 4; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(r[c + e]), __uint_as_float(r[c + e + 4]));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(r[BKV - 4 + e]));
+        const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+        // Lazy rescale: the maximum used moves only when the row's grows by more
+        // than 8 (weights stay <= 2^8); O and l move with it
+        const float m_new = fmaxf(m, top == -INFINITY ? -INFINITY : top * args.sc);
+        const bool grow = m_new > m + 8.0f;
+        if (grow) {
+          alpha = ex2(m - m_new);
+          m = m_new;
+        }
+        if (i > 0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll 1
+          for (int c = 0; c < DH; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_tm + c, o);
+            tmem_ld_wait();
+            tmem_reg_fence32(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st32(o_tm + c, o);
+          }
+        }
+        const float base = m == -INFINITY ? 0.0f : LIFT - m;  // nothing seen yet: every weight is 0
+        const uint64_t base2 = f2pack(base, base);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const int k = 64 * h + 2 * c;
+            float p0, p1;
+            f2unpack(f2fma(f2pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), sc2, base2), p0, p1);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            if (MASKED) {
+              if (k > seen) p0 = 0.0f;
+              if (k + 1 > seen) p1 = 0.0f;
+            }
+            sum2[c & 3] = f2add(sum2[c & 3], f2pack(p0, p1));
+            pk[c] = pack16<T>(p0, p1);
+          }
+          tmem_st32(s_tm + 32 * h, pk);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_half[2 * t + h]);
+        }
+      };
+      if (__any_sync(0xffffffffu, seen < BKV - 1))
+        block(std::true_type{});
+      else
+        block(std::false_type{});
       float a0, a1;
       f2unpack(f2add(f2add(sum2[0], sum2[1]), f2add(sum2[2], sum2[3])), a0, a1);
       l = l * alpha + (a0 + a1);
     }
     if (ok && my_n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_final[t], 0, abort_flag));
+    // splits of this tile that hold keys; with one the output is final
+    const int used = min(args.splits, max(1, (my_nkb + args.chunk - 1) / args.chunk));
+    const bool all_rows = used == 1 && blockIdx.z == 0 && *found && tok0 + (t + 1) * args.T <= pl.lq;
+    auto tile_sync = [&]() {  // the tile's four warps
+      if (t == 0)
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      else
+        asm volatile("bar.sync 2, 128;" ::: "memory");
+    };
     if (!ok) {
       if (lane == 0) {
         *abort_flag = 1;
         atomicCAS(&g_prompt_attn_err, 0, kErrTimeoutSoftmax);
       }
+      __syncwarp();
+      if (all_rows) tile_sync();  // the tile's other warps may be waiting there
     } else {
       // ---------------------------------------------------------------- epilogue
       tc_fence_after();
-      // splits of this tile that hold keys; with one the output is final
-      const int used = min(args.splits, max(1, (my_nkb + args.chunk - 1) / args.chunk));
       const bool mine = valid && static_cast<int>(blockIdx.z) < used;
       const float rl = l == 0.0f ? 0.0f : 1.0f / l;  // NaN stays NaN
       const int head = y * args.P + row % args.P;
       const long long qrow = pl.q0 + i_tok, slot = qrow * a.heads + head;
-      T* out = static_cast<T*>(a.out) + qrow * a.o_row + head * a.o_head;
       const long long part_rows = static_cast<long long>(a.total_q) * a.heads;
       float* part = args.part + (static_cast<long long>(blockIdx.z) * part_rows + slot) * DH;
       const bool patch = *any_bad != 0;
+      // the tile's Q is no longer read: its memory stages the outputs in Q's
+      // layout (pieces of a row swizzled)
+      uint8_t* stage = sQ + t * TILE + row * 128;
+      if (my_n > 0) {
 #pragma unroll 1
-      for (int c = 0; c < DH; c += 32) {
-        uint32_t o[32];
-        __syncwarp();
-        if (my_n > 0) {
-          tmem_ld32(o_tm + c, o);
+        for (int h = 0; h < NH; ++h) {
+          uint32_t o[64];
+          __syncwarp();
+          tmem_ld32(o_tm + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(o));
+          tmem_ld32(o_tm + 64 * h + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
           tmem_ld_wait();
-          tmem_reg_fence32(o);
-        }
-        if (!mine) continue;
+          tmem_reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(o));
+          tmem_reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(o + 32));
+          // l = 0: the row saw nothing
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[e]) * rl);
-        if (patch && l != 0.0f) {
-          for (int e = 0; e < 32; ++e) {
-            const bool nan = bad[c + e] <= lim, pos = bad[DH + c + e] <= lim, neg = bad[2 * DH + c + e] <= lim;
-            if (nan | (pos & neg)) o[e] = 0x7FFFFFFFu;
-            else if (pos | neg) o[e] = __float_as_uint(__uint_as_float(o[e]) + (pos ? INFINITY : -INFINITY));
+          for (int e = 0; e < 64; ++e) o[e] = l == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[e]) * rl);
+          if (patch && l != 0.0f) {
+            const int* first = bad + 64 * h;
+#pragma unroll
+            for (int e = 0; e < 64; ++e) {
+              const bool nan = first[e] <= lim, pos = first[DH + e] <= lim, neg = first[2 * DH + e] <= lim;
+              if (nan | (pos & neg)) o[e] = 0x7FFFFFFFu;
+              else if (pos | neg) o[e] = __float_as_uint(__uint_as_float(o[e]) + (pos ? INFINITY : -INFINITY));
+              asm volatile("" ::: "memory");  // one element's loads at a time: this path is rare, registers are not
+            }
           }
-        }
-        if (used > 1) {
+          if (used > 1) {
+            if (mine) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<uint4*>(part + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-        } else {
+              for (int e = 0; e < 64; e += 4)
+                *reinterpret_cast<uint4*>(part + 64 * h + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+          } else {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8)
-            if (c + e < a.head_dim)
-              *reinterpret_cast<uint4*>(out + c + e) =
+            for (int e = 0; e < 64; e += 8)
+              *reinterpret_cast<uint4*>(stage + h * HALF_BYTES + ((e >> 3) ^ (row & 7)) * 16) =
                   make_uint4(pack16<T>(__uint_as_float(o[e]), __uint_as_float(o[e + 1])),
                              pack16<T>(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])),
                              pack16<T>(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5])),
                              pack16<T>(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])));
+          }
+        }
+      } else if (mine) {  // no keys at all
+#pragma unroll
+        for (int e = 0; e < DH; e += 8)
+          *reinterpret_cast<uint4*>(stage + (e >> 6) * HALF_BYTES + (((e & 63) >> 3) ^ (row & 7)) * 16) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      const unsigned rows_out = __ballot_sync(0xffffffffu, mine && used == 1);
+      __syncwarp();
+      if (all_rows) {  // the tile's tokens all exist: one copy per half, in Q's layout
+        fence_proxy_async_smem();
+        tile_sync();
+        if (row == 0) {
+          for (int h = 0; h < NH; ++h)
+            if (64 * h < a.head_dim)
+              tma_store_4d(&args.tmO, sQ + t * TILE + h * HALF_BYTES, 64 * h, 0, pl.q0 + tok0 + t * args.T, y);
+          bulk_commit();
+          bulk_wait_read<0>();
+        }
+      } else if (rows_out) {
+        const long long at = qrow * a.o_row + head * a.o_head;
+        const uint8_t* base = sQ + t * TILE + quarter * 32 * 128;
+#pragma unroll 4
+        for (int r4 = 0; r4 < 32; r4 += 4) {
+          const int r = r4 + (lane >> 3), piece = lane & 7;
+          const long long off = __shfl_sync(0xffffffffu, at, r);
+          if (!((rows_out >> r) & 1u)) continue;
+          T* out = static_cast<T*>(a.out) + off + piece * 8;
+#pragma unroll
+          for (int h = 0; h < NH; ++h)
+            if (64 * h + piece * 8 < a.head_dim)
+              *reinterpret_cast<uint4*>(out + 64 * h) =
+                  *reinterpret_cast<const uint4*>(base + h * HALF_BYTES + r * 128 + (piece ^ (r & 7)) * 16);
         }
       }
       if (mine && used > 1) args.ml[static_cast<long long>(blockIdx.z) * part_rows + slot] = make_float2(m, l);
@@ -718,7 +785,7 @@ int prompt_attention_launch(const PromptAttnArgs& a, cudaStream_t stream) {
   d.chunk = p.chunk;
   d.splits = p.splits;
   d.sc = (a.scale < 0.0f ? -a.scale : a.scale) * 1.4426950408889634f;
-  d.negate = a.scale < 0.0f;
+  d.negate = a.scale < 0.0f ? 1u << 13 : 0u;
   if (p.splits > 1) {
     const long long rows = static_cast<long long>(a.total_q) * a.heads;
     d.part = static_cast<float*>(a.workspace);
@@ -727,13 +794,15 @@ int prompt_attention_launch(const PromptAttnArgs& a, cudaStream_t stream) {
   // a dimension of one element has no stride to go by: any valid one will do
   auto stride = [](long long s, long long n) { return static_cast<cuuint64_t>(n > 1 ? s * 2 : 16); };
   const cuuint64_t dim = a.head_dim;
-  {  // Q: (d, head of the pack, token, pack): a tile's rows are token-major, heads inside
+  // Q, out: (d, head of the pack, token, pack): a tile's rows are token-major, heads inside
+  auto rows = [&](CUtensorMap* tm, const void* base, long long row, long long head) {
     cuuint64_t dims[4] = {dim, static_cast<cuuint64_t>(p.P), static_cast<cuuint64_t>(a.total_q),
                           static_cast<cuuint64_t>(a.heads / p.P)};
-    cuuint64_t str[3] = {stride(a.q_head, p.P), stride(a.q_row, a.total_q), stride(a.q_head * p.P, a.heads / p.P)};
+    cuuint64_t str[3] = {stride(head, p.P), stride(row, a.total_q), stride(head * p.P, a.heads / p.P)};
     cuuint32_t box[4] = {64, static_cast<cuuint32_t>(p.P), static_cast<cuuint32_t>(p.T), 1};
-    if (encode_heads(&d.tmQ, a.dtype, a.q, 4, dims, str, box) != QI_OK) return QI_ERR_CUDA;
-  }
+    return encode_heads(tm, a.dtype, base, 4, dims, str, box);
+  };
+  if (rows(&d.tmQ, a.q, a.q_row, a.q_head) != QI_OK || rows(&d.tmO, a.out, a.o_row, a.o_head) != QI_OK) return QI_ERR_CUDA;
   // K, V: (d, kv head, row); without rows the base is never read, and any will do
   auto kv = [&](CUtensorMap* tm, const void* base, long long row, long long head) {
     cuuint64_t dims[3] = {dim, static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.total_k > 0 ? a.total_k : 1)};
