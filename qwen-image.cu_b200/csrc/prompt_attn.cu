@@ -423,7 +423,8 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
     const int my_n = NT == 1 || t == 0 ? n[0] : n[NT - 1], my_nkb = NT == 1 || t == 0 ? nkb[0] : nkb[NT - 1];
     const int tok = row / args.P, i_tok = tok0 + t * args.T + tok;  // token in its sequence
     const bool valid = *found && tok < args.T && i_tok < pl.lq;
-    const int lim = valid ? last_seen(i_tok, pl.lq, pl.lk, a.causal) : -1;
+    // rows that are no query (their results go nowhere) do not ask for masking
+    const int lim = valid ? last_seen(i_tok, pl.lq, pl.lk, a.causal) : lim_unit;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_tm = tmem + lane_off + 128 * t, o_tm = tmem + lane_off + 128 * (NT + t);
     // FP16 weights are kept in 2^7 .. 2^15 for the largest so that small ones
@@ -453,7 +454,7 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
         if (MASKED) {
 #pragma unroll
           for (int c = 0; c < BKV; ++c)
-            if (c > seen) r[c] = 0xFF800000u;  // -inf
+            if (c > seen) r[c] = 0xFF800000u;  // -inf: weight 0
         }
         float mx[4];
 #pragma unroll
@@ -497,10 +498,6 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
             f2unpack(f2fma(f2pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), sc2, base2), p0, p1);
             p0 = ex2(p0);
             p1 = ex2(p1);
-            if (MASKED) {
-              if (k > seen) p0 = 0.0f;
-              if (k + 1 > seen) p1 = 0.0f;
-            }
             sum2[c & 3] = f2add(sum2[c & 3], f2pack(p0, p1));
             pk[c] = pack16<T>(p0, p1);
           }
@@ -785,6 +782,9 @@ int prompt_attention_launch(const PromptAttnArgs& a, cudaStream_t stream) {
   d.chunk = p.chunk;
   d.splits = p.splits;
   d.sc = (a.scale < 0.0f ? -a.scale : a.scale) * 1.4426950408889634f;
+  // scale 0: the smallest normal number does the same to finite scores (every
+  // weight 1) and leaves masked ones at -inf, where 0 would make them NaN
+  if (d.sc < 1.17549435e-38f) d.sc = 1.17549435e-38f;
   d.negate = a.scale < 0.0f ? 1u << 13 : 0u;
   if (p.splits > 1) {
     const long long rows = static_cast<long long>(a.total_q) * a.heads;
