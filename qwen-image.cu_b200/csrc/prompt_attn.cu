@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
   uint64_t* v_ready = v_full + VS;     // [VS] the V guard has passed the block (2 warps)
   uint64_t* v_empty = v_ready + VS;    // [VS]
   uint64_t* s_full = v_empty + VS;     // [NT] QK of the tile's current block complete
-  uint64_t* s_loaded = s_full + NT;    // [NT] the tile's S is in registers (4 warps)
+  uint64_t* s_loaded = s_full + NT;    // [NT] the tile's S is in registers (4 warps; one-tile CTAs)
   uint64_t* p_half = s_loaded + NT;    // [NT][2] half h of the tile's P is in TMEM (4 warps)
   uint64_t* o_final = p_half + 2 * NT; // [NT] the tile's last PV complete
   uint64_t* drain = o_final + NT;
@@ -326,6 +326,14 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
           }
           mma_commit_elect(&k_empty[0]);
         }
+        // P occupies half of S_t's columns, so the next block's product goes
+        // behind P_t V; a CTA's MMAs run in issue order.  With two tiles it is
+        // one N = 128 product (the other tile's work fills the time; 8192 causal
+        // tokens: 454 us against 484 us with halves).  With one, its upper half
+        // of keys, whose columns never hold P, goes ahead as soon as S_t has been
+        // read (N = 64 products re-read Q twice as often, but nothing else wants
+        // the tensor cores: 16 caches of up to 4096, 34.6 against 35.7 us).
+        constexpr bool EARLY = NT == 1;
         for (int i = 0; i < nmax && ok; ++i) {
           const int vs = i % VS, ks = (i + 1) % KS;
           const uint32_t vp = (i / VS) & 1, kp = ((i + 1) / KS) & 1;
@@ -335,7 +343,7 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
             const bool more = i + 1 < n[t];
             // the last tile that still uses this V block / the next K block
             const bool last_v = t == NT - 1 || i >= n[NT - 1], last_k = t == NT - 1 || i + 1 >= n[NT - 1];
-            if (more) {  // upper half of S_t for the next block: its columns never hold P
+            if (more && EARLY) {
               ok = wait_all(&s_loaded[t], i & 1) && wait_all(&k_full[ks], kp);
               if (!ok) break;
               tc_fence_after();
@@ -352,9 +360,14 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
             if (!more) mma_commit_elect(&o_final[t]);
             if (last_v) mma_commit_elect(&v_empty[vs]);
             if (more) {
-              // the lower half overwrites the columns P_t V reads: it is issued
-              // behind it, and a CTA's MMAs run in issue order
-              qk_half(t, ks, 0);
+              if (EARLY) {
+                qk_half(t, ks, 0);
+              } else {
+                ok = wait_all(&k_full[ks], kp);
+                if (!ok) break;
+                tc_fence_after();
+                qk(t, ks);
+              }
               mma_commit_elect(&s_full[t]);
               if (last_k) mma_commit_elect(&k_empty[ks]);
             }
@@ -443,9 +456,11 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
       tmem_ld_wait();
 #pragma unroll
       for (int c = 0; c < BKV; c += 32) tmem_reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(r + c));
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_loaded[t]);
+      if (NT == 1) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_loaded[t]);
+      }
       const int key0 = (jb + i) * BKV, seen = lim - key0;  // keys 0 .. seen of the block are seen
       float alpha = 1.0f;
       uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
