@@ -10,7 +10,8 @@
 // 128): row = token in tile * P + head.  K and V are read once for the group,
 // and a causal tile spans few positions, so little of its last key block is
 // masked.  A CTA runs NT tiles over one K / V stream; with few tiles the keys
-// are also split over blockIdx.z and a second kernel joins the parts.
+// are also split, by the actual lengths (every CTA works out the same division
+// from them), and a second kernel joins the parts.
 //
 // A CTA's warps: 0 TMA producer, 1 MMA issuer, 2-3 the V guard (below), then a
 // warpgroup of softmax threads per tile (thread = row = TMEM lane).  Per 128-key
@@ -36,6 +37,7 @@ namespace {
 __device__ int g_prompt_attn_err;  // set by a bounded wait that gave up (prompt_attention_take_error)
 
 constexpr int BQ = 128, BKV = 128;
+constexpr int CACHED_SEQS = 256;  // sequences whose ranges a CTA keeps in shared memory
 constexpr int HALF_BYTES = 128 * 128;  // 128 rows x 64 elements: one swizzled box column
 
 template <int DH, int NT>
@@ -49,7 +51,7 @@ struct Cfg {
   static_assert(128 * PRODUCER_REGS + 128 * NT * SOFTMAX_REGS <= THREADS * LAUNCH_REGS, "register split exceeds the launch");
   static constexpr int TILE = NH * HALF_BYTES;  // Q tile, K block or V block
   static constexpr int OFF_K = NT * TILE, OFF_V = OFF_K + KS * TILE, OFF_X = OFF_V + VS * TILE;
-  static constexpr int SMEM = 1024 + OFF_X + 2048;
+  static constexpr int SMEM = 1024 + OFF_X + 2048 + 16 * CACHED_SEQS;
   static constexpr int TMEM_COLS = 256 * NT;  // S of tile t at 128 t, O at 128 (NT + t)
 };
 
@@ -57,12 +59,14 @@ struct alignas(64) PromptAttnDev {
   CUtensorMap tmQ, tmK, tmV, tmO;
   PromptAttnArgs a;
   int P, T, packs;   // heads per tile row group, tokens per tile, tiles' head packs per kv head
-  int units;         // upper bound of NT-tile units over all sequences (gridDim.x)
-  int chunk, splits;  // key blocks per split; gridDim.z
+  int items;         // work items per head pack at most: (unit of NT tiles, split of its keys) (gridDim.x)
+  int splits;        // splits of a sequence's keys at most
+  int join_warps;    // warps per row of the joining kernel
   float sc;          // |scale| log2(e)
   uint32_t negate;   // scale < 0: instruction descriptor bit 13 (negate A) for Q K^T
   float* part;       // splits > 1: [splits][total_q * heads][DH] normalised partial outputs
   float2* ml;        // splits > 1: [splits][total_q * heads] (m, l)
+  int* used;         // splits > 1: [total_q * heads] splits that hold the row's keys
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -93,27 +97,93 @@ __device__ __forceinline__ uint32_t pack16<__half>(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
-// The sequence that holds unit `u` when every sequence has ceil(Lq / step)
-// units in order, and the unit's index in it; false past the last.  Called by
-// one whole warp.
-struct Place {
-  int seq, unit, q0, lq, k0, lk;
-};
-__device__ __forceinline__ bool clip(const PromptAttnArgs& a, int b, Place& p) {
-  p.q0 = min(max(a.q_begin[b], 0), a.total_q);
-  p.lq = min(max(a.q_end[b], p.q0), a.total_q) - p.q0;
-  p.k0 = min(max(a.k_begin[b], 0), a.total_k);
-  p.lk = min(max(a.k_end[b], p.k0), a.total_k) - p.k0;
-  return true;
+// Last key (relative to the sequence) that token i of the sequence sees, or -1.
+__device__ __forceinline__ int last_seen(int i, int lq, int lk, int causal) {
+  return causal ? max(min(i + lk - lq, lk - 1), -1) : lk - 1;
 }
-__device__ __forceinline__ bool find_unit(const PromptAttnArgs& a, int step, int u, Place& out) {
+
+// A sequence's ranges, clipped to the tensors: (q0, Lq, k0, Lk).
+__device__ __forceinline__ int4 sequence(const PromptAttnArgs& a, int b) {
+  const int q0 = a.q_begin[b], q1 = a.q_end[b], k0 = a.k_begin[b], k1 = a.k_end[b];
+  int4 p;
+  p.x = min(max(q0, 0), a.total_q);
+  p.y = min(max(q1, p.x), a.total_q) - p.x;
+  p.z = min(max(k0, 0), a.total_k);
+  p.w = min(max(k1, p.z), a.total_k) - p.z;
+  return p;
+}
+// A work item: the unit-th step of a sequence's tokens, the split-th part of its keys.
+struct Place {
+  int q0, lq, k0, lk;
+  int unit, split;
+};
+// Units of `step` tokens of a sequence, and key blocks of its last one.
+__device__ __forceinline__ int units_of(int4 p, int step) { return (p.y + step - 1) / step; }
+__device__ __forceinline__ int blocks_of(int4 p, int causal) {
+  return p.y > 0 ? (last_seen(p.y - 1, p.y, p.w, causal) + BKV) / BKV : 0;
+}
+__device__ __forceinline__ int splits_of(int blocks, int chunk) { return max(1, (blocks + chunk - 1) / chunk); }
+
+// Key blocks per split: the smallest number that keeps all sequences' work items
+// within args.items (whole waves of CTAs) and a sequence's splits within
+// args.splits; every CTA of the call works out the same.  Called by a whole CTA;
+// leaves the first CACHED_SEQS sequences in `seqs`.
+__device__ __forceinline__ int chunk_of(const PromptAttnDev& d, int step, int* smem, int4* seqs) {
+  const PromptAttnArgs& a = d.a;
+  const int tid = threadIdx.x, nt = blockDim.x;
+  int *total = smem, *longest = smem + 1, *count = smem + 2;  // count: two, taking turns
+  if (tid < 4) smem[tid] = 0;
+  const bool split = d.splits > 1;
+  if (split) __syncthreads();
+  int u0 = 0, n0 = 0;  // this thread's first sequence
+  for (int b = tid; b < a.batch; b += nt) {
+    const int4 p = sequence(a, b);
+    if (b < CACHED_SEQS) seqs[b] = p;
+    if (!split) {
+      if (b + nt >= CACHED_SEQS) break;
+      continue;
+    }
+    const int u = units_of(p, step), n = blocks_of(p, a.causal);
+    if (b == tid) {
+      u0 = u;
+      n0 = n;
+    }
+    // (a count that saturates only makes the first guess of the chunk smaller)
+    atomicAdd(total, static_cast<int>(min(static_cast<long long>(u) * n, 1ll << 20)));
+    atomicMax(longest, n);
+  }
+  __syncthreads();
+  if (!split) return INT_MAX / 2;
+  const int most = *longest;
+  int chunk = max(max(2, (most + d.splits - 1) / d.splits), min(max(*total, 0) / d.items, most));
+  for (int turn = 0; chunk < most; turn ^= 1) {
+    int mine = tid < a.batch ? u0 * splits_of(n0, chunk) : 0;
+    for (int b = tid + nt; b < a.batch; b += nt) {
+      const int4 p = sequence(a, b);
+      mine += units_of(p, step) * splits_of(blocks_of(p, a.causal), chunk);
+    }
+    if (mine) atomicAdd(count + turn, mine);
+    __syncthreads();
+    const bool fits = count[turn] <= d.items;
+    if (tid == 0) count[turn ^ 1] = 0;
+    __syncthreads();
+    if (fits) break;
+    chunk += max(1, chunk / 8);
+  }
+  return chunk;
+}
+
+// Work item `u` when the sequences' items follow one another; false past the
+// last.  Called by one whole warp.
+__device__ __forceinline__ bool find_item(const PromptAttnArgs& a, int step, int chunk, int u, const int4* seqs, Place& out) {
   const int lane = threadIdx.x & 31;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    Place p = {};
-    int n = 0;
+    int4 p = make_int4(0, 0, 0, 0);
+    int n = 0, s = 1;
     if (b0 + lane < a.batch) {
-      clip(a, b0 + lane, p);
-      n = (p.lq + step - 1) / step;
+      p = b0 + lane < CACHED_SEQS ? seqs[b0 + lane] : sequence(a, b0 + lane);
+      s = splits_of(blocks_of(p, a.causal), chunk);
+      n = units_of(p, step) * s;
     }
     int sum = n;  // inclusive prefix sum over the lanes
 #pragma unroll
@@ -124,22 +194,18 @@ __device__ __forceinline__ bool find_unit(const PromptAttnArgs& a, int step, int
     const unsigned hit = __ballot_sync(0xffffffffu, u < sum);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      out.seq = b0 + src;
-      out.unit = u - __shfl_sync(0xffffffffu, sum - n, src);
-      out.q0 = __shfl_sync(0xffffffffu, p.q0, src);
-      out.lq = __shfl_sync(0xffffffffu, p.lq, src);
-      out.k0 = __shfl_sync(0xffffffffu, p.k0, src);
-      out.lk = __shfl_sync(0xffffffffu, p.lk, src);
+      const int r = u - __shfl_sync(0xffffffffu, sum - n, src), sp = __shfl_sync(0xffffffffu, s, src);
+      out.q0 = __shfl_sync(0xffffffffu, p.x, src);
+      out.lq = __shfl_sync(0xffffffffu, p.y, src);
+      out.k0 = __shfl_sync(0xffffffffu, p.z, src);
+      out.lk = __shfl_sync(0xffffffffu, p.w, src);
+      out.unit = r / sp;
+      out.split = r % sp;
       return true;
     }
     u -= __shfl_sync(0xffffffffu, sum, 31);
   }
   return false;
-}
-
-// Last key (relative to the sequence) that token i of the sequence sees, or -1.
-__device__ __forceinline__ int last_seen(int i, int lq, int lk, int causal) {
-  return causal ? max(min(i + lk - lq, lk - 1), -1) : lk - 1;
 }
 
 template <typename T>
@@ -174,6 +240,8 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
   int* any_bad = const_cast<int*>(abort_flag) + 1;
   Place* place = reinterpret_cast<Place*>(any_bad + 1);
   int* found = reinterpret_cast<int*>(place + 1);
+  int* sched = found + 1;  // chunk_of's four words
+  int4* seqs = reinterpret_cast<int4*>(smem + C::OFF_X + 2048);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PromptAttnArgs& a = args.a;
@@ -212,9 +280,10 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
     for (int i = lane; i < 3 * DH; i += 32) bad[i] = INT_MAX;
   grid_dependency_wait();
   launch_dependents();
-  if (warp == 0) {  // units in descending order: a causal sequence's later units have more keys
-    Place p;
-    const bool ok = find_unit(a, NT * args.T, args.units - 1 - static_cast<int>(blockIdx.x), p);
+  const int chunk = chunk_of(args, NT * args.T, sched, seqs);
+  if (warp == 0) {  // in descending order: a causal sequence's later units have more keys
+    Place p = {};
+    const bool ok = find_item(a, NT * args.T, chunk, args.items - 1 - static_cast<int>(blockIdx.x), seqs, p);
     if (lane == 0) {
       *place = p;
       *found = ok;
@@ -228,12 +297,12 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
   const int tok0 = pl.unit * NT * args.T;  // first token of the unit in its sequence
   // key blocks [jb, je[t]) of tile t in this split; n[t] of them
   int n[NT], nkb[NT], nmax = 0;
-  const int jb = static_cast<int>(blockIdx.z) * args.chunk;
+  const int jb = pl.split * chunk;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int first = tok0 + t * args.T, lim = last_seen(min(first + args.T, pl.lq) - 1, pl.lq, pl.lk, a.causal);
     nkb[t] = *found && first < pl.lq ? (lim + BKV) / BKV : 0;  // lim = -1: none
-    const int je = static_cast<int>(blockIdx.z) == args.splits - 1 ? nkb[t] : min(nkb[t], jb + args.chunk);
+    const int je = min(nkb[t], jb + chunk);
     n[t] = max(0, je - jb);
     nmax = max(nmax, n[t]);
   }
@@ -533,8 +602,8 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
     }
     if (ok && my_n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_final[t], 0, abort_flag));
     // splits of this tile that hold keys; with one the output is final
-    const int used = min(args.splits, max(1, (my_nkb + args.chunk - 1) / args.chunk));
-    const bool all_rows = used == 1 && blockIdx.z == 0 && *found && tok0 + (t + 1) * args.T <= pl.lq;
+    const int used = splits_of(my_nkb, chunk);
+    const bool all_rows = used == 1 && pl.split == 0 && *found && tok0 + (t + 1) * args.T <= pl.lq;
     auto tile_sync = [&]() {  // the tile's four warps
       if (t == 0)
         asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -551,12 +620,12 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
     } else {
       // ---------------------------------------------------------------- epilogue
       tc_fence_after();
-      const bool mine = valid && static_cast<int>(blockIdx.z) < used;
+      const bool mine = valid && pl.split < used;
       const float rl = l == 0.0f ? 0.0f : 1.0f / l;  // NaN stays NaN
       const int head = y * args.P + row % args.P;
       const long long qrow = pl.q0 + i_tok, slot = qrow * a.heads + head;
       const long long part_rows = static_cast<long long>(a.total_q) * a.heads;
-      float* part = args.part + (static_cast<long long>(blockIdx.z) * part_rows + slot) * DH;
+      float* part = args.part + (static_cast<long long>(pl.split) * part_rows + slot) * DH;
       const bool patch = *any_bad != 0;
       // the tile's Q is no longer read: its memory stages the outputs in Q's
       // layout (pieces of a row swizzled)
@@ -633,7 +702,8 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
                   *reinterpret_cast<const uint4*>(base + h * HALF_BYTES + r * 128 + (piece ^ (r & 7)) * 16);
         }
       }
-      if (mine && used > 1) args.ml[static_cast<long long>(blockIdx.z) * part_rows + slot] = make_float2(m, l);
+      if (mine && pl.split == 0 && args.splits > 1) args.used[slot] = used;
+      if (mine && used > 1) args.ml[static_cast<long long>(pl.split) * part_rows + slot] = make_float2(m, l);
     }
   }
 
@@ -646,63 +716,85 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
 }
 
 // Joins the splits of a row: out = sum_s w_s O_s / sum_s w_s, w_s = l_s 2^(m_s - max m).
-// One warp per (token, head), four dimensions per thread; rows whose tile had
-// one split are final already.
+// A CTA per token and 8 / per heads; `per` warps per head take its splits in
+// turn, four dimensions per thread, and add up in warp order.  Rows whose tile
+// had one split are final already.
 template <typename T, int DH>
 __global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_constant__ PromptAttnDev args) {
+  __shared__ float4 part_o[8][32];
+  __shared__ float2 part_w[8];
   grid_dependency_wait();
   launch_dependents();
   const PromptAttnArgs& a = args.a;
-  const int lane = threadIdx.x & 31;
-  const long long slot = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = args.join_warps, wi = warp % per;
+  const int qrow = blockIdx.x, head = blockIdx.y * (8 / per) + warp / per;
   const long long rows = static_cast<long long>(a.total_q) * a.heads;
-  if (slot >= rows) return;
-  const int qrow = static_cast<int>(slot / a.heads), head = static_cast<int>(slot % a.heads);
-  Place p = {};
+  const long long slot = static_cast<long long>(qrow) * a.heads + head;
+  // read ahead of the look-up; means nothing for a row of no sequence
+  int used = head < a.heads ? args.used[slot] : 0;
   bool found = false;
   for (int b0 = 0; b0 < a.batch && !found; b0 += 32) {
-    Place c = {};
     bool hit = false;
-    if (b0 + lane < a.batch) {
-      clip(a, b0 + lane, c);
-      hit = qrow >= c.q0 && qrow < c.q0 + c.lq;
-    }
-    const unsigned m = __ballot_sync(0xffffffffu, hit);
-    if (m) {
-      found = true;
-      const int src = __ffs(m) - 1;
-      p.q0 = __shfl_sync(0xffffffffu, c.q0, src);
-      p.lq = __shfl_sync(0xffffffffu, c.lq, src);
-      p.lk = __shfl_sync(0xffffffffu, c.lk, src);
-    }
+    if (b0 + lane < a.batch) hit = qrow >= a.q_begin[b0 + lane] && qrow < a.q_end[b0 + lane];
+    found = __any_sync(0xffffffffu, hit);
   }
-  if (!found) return;
-  const int tile_end = min(((qrow - p.q0) / args.T + 1) * args.T, p.lq) - 1;
-  const int nkb = (last_seen(tile_end, p.lq, p.lk, a.causal) + BKV) / BKV;
-  const int used = min(args.splits, max(1, (nkb + args.chunk - 1) / args.chunk));
-  if (used <= 1 || 4 * lane >= DH) return;
-  float top = -INFINITY;
-  for (int s = 0; s < used; ++s) top = fmaxf(top, args.ml[s * rows + slot].x);
+  const bool work = found && head < a.heads && used > 1;
+  // this warp's splits: wi, wi + per, ...; lane i holds the i-th's (m, l)
+  const int mine = work && wi < used ? (used - wi + per - 1) / per : 0;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float total = 0.0f;
-  for (int s = 0; s < used; ++s) {
-    const float2 ml = args.ml[s * rows + slot];
-    if (ml.y == 0.0f) continue;  // this part saw nothing
-    const float w = ml.y * ex2(ml.x - top);
-    const float4 v = *reinterpret_cast<const float4*>(args.part + (s * rows + slot) * DH + 4 * lane);
-    total += w;
-    o = make_float4(o.x + w * v.x, o.y + w * v.y, o.z + w * v.z, o.w + w * v.w);
+  float total = 0.0f, top = -INFINITY;
+  for (int i0 = 0; i0 < mine; i0 += 32) {
+    const long long s = wi + static_cast<long long>(i0 + lane) * per;
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (i0 + lane < mine) ml = args.ml[s * rows + slot];
+    float t = ml.y == 0.0f ? -INFINITY : ml.x;  // l = 0: this part saw nothing
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
+    t = fmaxf(t, top);
+    const float keep = top == -INFINITY ? 0.0f : ex2(top - t);
+    top = t;
+    total *= keep;
+    o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+    const float w_lane = ml.y == 0.0f ? 0.0f : ml.y * ex2(ml.x - top);
+#pragma unroll 4
+    for (int i = 0; i < min(mine - i0, 32); ++i) {
+      const float w = __shfl_sync(0xffffffffu, w_lane, i);
+      if (w == 0.0f || 4 * lane >= DH) continue;
+      const float4 v = *reinterpret_cast<const float4*>(
+          args.part + ((wi + static_cast<long long>(i0 + i) * per) * rows + slot) * DH + 4 * lane);
+      total += w;
+      o = make_float4(o.x + w * v.x, o.y + w * v.y, o.z + w * v.z, o.w + w * v.w);
+    }
+    total = __shfl_sync(0xffffffffu, total, 0);
   }
+  if (per > 1) {
+    part_o[warp][lane] = o;
+    if (lane == 0) part_w[warp] = make_float2(top, total);
+    __syncthreads();
+    if (wi != 0) return;
+    for (int i = 0; i < per; ++i) top = fmaxf(top, part_w[warp + i].x);
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    total = 0.0f;
+    for (int i = 0; i < per; ++i) {
+      const float2 tw = part_w[warp + i];
+      if (tw.x == -INFINITY && tw.y == 0.0f) continue;
+      const float k = ex2(tw.x - top);
+      const float4 v = part_o[warp + i][lane];
+      total += k * tw.y;
+      o = make_float4(o.x + k * v.x, o.y + k * v.y, o.z + k * v.z, o.w + k * v.w);
+    }
+  }
+  if (!work || 4 * lane >= a.head_dim) return;
   const float r = total == 0.0f ? 0.0f : 1.0f / total;
-  if (4 * lane >= a.head_dim) return;
   T* out = static_cast<T*>(a.out) + qrow * a.o_row + head * a.o_head + 4 * lane;
   *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(o.x * r, o.y * r), pack16<T>(o.z * r, o.w * r));
 }
 
 // ------------------------------------------------------------------ host
 struct Plan {
-  int P, T, packs, nt, chunk, splits, dh;
-  long long units;
+  int P, T, packs, nt, splits, dh;
+  long long items;
 };
 
 Plan plan_of(int heads, int kv_heads, int head_dim, int batch, int total_q, int max_k, int num_sms) {
@@ -713,20 +805,22 @@ Plan plan_of(int heads, int kv_heads, int head_dim, int batch, int total_q, int 
   while (p.P > BQ || G % p.P) --p.P;
   p.T = BQ / p.P;
   p.packs = G / p.P;
-  const long long ctas1 = (static_cast<long long>(total_q) / p.T + batch) * (heads / p.P);
-  // one tile per CTA while those fit on the device at once (shorter calls), two
-  // over one K / V stream beyond that
-  p.nt = ctas1 <= num_sms ? 1 : 2;
-  p.units = static_cast<long long>(total_q) / (p.nt * p.T) + batch;
-  const long long ctas = p.units * (heads / p.P);
-  const int blocks = max_k / BKV + (max_k % BKV != 0);
-  // key splits: fill the device (two CTAs per SM with heads of 64)
+  const long long groups = heads / p.P;
+  // One tile per CTA while those fit on the device at once (shorter calls) or
+  // sequences fill no second one; two over one K / V stream beyond that
+  const long long ctas1 = (static_cast<long long>(total_q) / p.T + batch) * groups;
+  p.nt = ctas1 <= num_sms || total_q < 2ll * p.T * batch ? 1 : 2;
+  const long long units = static_cast<long long>(total_q) / (p.nt * p.T) + batch, ctas = units * groups;
+  // Key splits while the units alone leave the device (two CTAs per SM with
+  // heads of 64) short of work, or, one token each, of even work; at least two
+  // blocks each.  More than 4 (2) x the CTAs it holds would only cost workspace.
   const long long slots = static_cast<long long>(num_sms) * (p.nt == 1 && p.dh == 64 ? 2 : 1);
-  long long splits = ctas < slots ? slots / ctas : 1;
-  if (splits > (blocks + 1) / 2) splits = (blocks + 1) / 2;  // two blocks each at least
-  if (splits < 1) splits = 1;
-  p.chunk = blocks > 0 ? static_cast<int>((blocks + splits - 1) / splits) : 1;
-  p.splits = blocks > 0 ? (blocks + p.chunk - 1) / p.chunk : 1;
+  long long splits = (p.nt == 1 ? 4 : 2) * slots / ctas;
+  const int blocks = max_k / BKV + (max_k % BKV != 0);
+  if (splits > blocks / 2) splits = blocks / 2;
+  p.splits = splits < 1 ? 1 : static_cast<int>(splits);
+  const long long wave = slots / groups < 1 ? 1 : slots / groups;  // work items per head group that run at once
+  p.items = p.splits > 1 ? (units + wave - 1) / wave * wave : units;
   return p;
 }
 
@@ -762,11 +856,12 @@ int launch_tiles(const PromptAttnDev& d, cudaStream_t stream) {
   static unsigned long long attr_done = 0;
   const auto fn = prompt_attn_kernel<T, DH, NT>;
   if (smem_optin(reinterpret_cast<const void*>(fn), C::SMEM, &attr_done) != QI_OK) return QI_ERR_CUDA;
-  const dim3 grid(d.units, d.a.heads / d.P, d.splits);
+  const dim3 grid(d.items, d.a.heads / d.P);
   const int st = launch_dependent(fn, grid, C::THREADS, C::SMEM, d, stream);
   if (st != QI_OK || d.splits == 1) return st;
-  const long long rows = static_cast<long long>(d.a.total_q) * d.a.heads;
-  return launch_dependent(prompt_attn_join_kernel<T, DH>, dim3(static_cast<unsigned>((rows + 7) / 8)), 256, 0, d, stream);
+  const int per_cta = 8 / d.join_warps;
+  return launch_dependent(prompt_attn_join_kernel<T, DH>, dim3(d.a.total_q, (d.a.heads + per_cta - 1) / per_cta), 256, 0, d,
+                          stream);
 }
 
 template <typename T>
@@ -781,21 +876,21 @@ long long prompt_attention_workspace(int heads, int kv_heads, int head_dim, int 
   if (batch == 0 || total_q == 0) return 0;
   const Plan p = plan_of(heads, kv_heads, head_dim, batch, total_q, max_k, device_num_sms());
   if (p.splits == 1) return 0;
-  return static_cast<long long>(p.splits) * total_q * heads * (p.dh * 4 + 8);
+  return static_cast<long long>(total_q) * heads * (p.splits * (p.dh * 4ll + 8) + 4);
 }
 
 int prompt_attention_launch(const PromptAttnArgs& a, cudaStream_t stream) {
   const Plan p = plan_of(a.heads, a.kv_heads, a.head_dim, a.batch, a.total_q, a.max_k, device_num_sms());
-  if (p.units > 0x7fffffffll) return QI_ERR_UNSUPPORTED;
+  if (p.items > 0x7fffffffll) return QI_ERR_UNSUPPORTED;
   PromptAttnDev d;
   memset(&d, 0, sizeof(d));
   d.a = a;
   d.P = p.P;
   d.T = p.T;
   d.packs = p.packs;
-  d.units = static_cast<int>(p.units);
-  d.chunk = p.chunk;
+  d.items = static_cast<int>(p.items);
   d.splits = p.splits;
+  d.join_warps = p.splits >= 16 ? 8 : (p.splits >= 8 ? 4 : (p.splits >= 4 ? 2 : 1));
   d.sc = (a.scale < 0.0f ? -a.scale : a.scale) * 1.4426950408889634f;
   // scale 0: the smallest normal number does the same to finite scores (every
   // weight 1) and leaves masked ones at -inf, where 0 would make them NaN
@@ -805,6 +900,7 @@ int prompt_attention_launch(const PromptAttnArgs& a, cudaStream_t stream) {
     const long long rows = static_cast<long long>(a.total_q) * a.heads;
     d.part = static_cast<float*>(a.workspace);
     d.ml = reinterpret_cast<float2*>(d.part + p.splits * rows * p.dh);
+    d.used = reinterpret_cast<int*>(d.ml + p.splits * rows);
   }
   // a dimension of one element has no stride to go by: any valid one will do
   auto stride = [](long long s, long long n) { return static_cast<cuuint64_t>(n > 1 ? s * 2 : 16); };
