@@ -110,8 +110,17 @@ __device__ __forceinline__ void add_bias32(float (&v)[32], const T* p, int n_val
 namespace pk {
 constexpr int BM = 256, BN_MAX = 256;
 constexpr int A_BYTES = 128 * BK * 2;  // this CTA's 128 rows of x
-constexpr int PROD_WARPS = 2, EPI_WARPS = 8;
-constexpr int THREADS = 32 * (PROD_WARPS + 1 + EPI_WARPS);
+constexpr int MMA_WARP = 2, EPI_WARP0 = 3, EPI_WARPS = 8;  // warps 0 and 1 produce
+constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS);
+// Long sums (FP32 outputs, K > 4096).  The tensor cores round every addition to
+// an accumulator towards zero, so its error grows with K: measured 1.6e-5 of the
+// product at K = 14336.  There the epilogue warps take the accumulator over every
+// 2048 of K and add it, rounding to nearest, to a sum that also lives in TMEM
+// (error as at K = 2048: 2e-6).  Two accumulators and the sum are 3 x 160 of the
+// 512 columns, so these tiles are at most 160 wide (SwiGLU: 128).  16-bit outputs
+// do not see the error.
+constexpr int SUMS_MIN_K = 4096, SUMS_STEP = 2048 / BK;
+constexpr int SUMS_BN = 160, SUMS_BN_WIDE = 128;
 // staging sub-tile of one epilogue warp: 32 rows x 32 columns of the output
 template <typename O>
 constexpr int sub_bytes() { return 32 * 32 * static_cast<int>(sizeof(O)); }
@@ -131,11 +140,12 @@ __device__ __forceinline__ void pair_tile(const L16Dev& a, int t, int& m0, int& 
   n0 = r / rows;  // column tile index
 }
 
-template <typename T, typename O>
+template <typename T, typename O, bool SUMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
     linear16_pair_kernel(const __grid_constant__ L16Dev args) {
   using namespace pk;
   constexpr int SUB = sub_bytes<O>();
+  constexpr int ACC = SUMS ? SUMS_BN : BN_MAX;  // TMEM columns of an accumulator; SUMS: the sum at 2 ACC
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int stages = args.stages, b_bytes = args.bn / 2 * BK * 2;  // b: this CTA's half of the tile's w rows
@@ -159,6 +169,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
   const bool wide = args.act == QI_ACT_SWIGLU;
   const int bn_out = wide ? bn / 2 : bn;
   const int kblocks = (args.K + BK - 1) / BK;
+  const int kstep = SUMS ? SUMS_STEP : kblocks;  // K blocks per accumulator
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
@@ -178,7 +189,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
     tma_prefetch_desc(&args.tmO);
     if (args.residual) tma_prefetch_desc(&args.tmR);
   }
-  if (warp == PROD_WARPS) {
+  if (warp == MMA_WARP) {
     tmem_alloc_pair(tmem_slot, 512);
     tmem_relinquish_pair();
   }
@@ -190,7 +201,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
   grid_dependency_wait();
   launch_dependents();
 
-  if (warp < PROD_WARPS) {
+  if (warp < MMA_WARP) {
     // ------------------------------------------------------------ producers (both CTAs)
     // Warp 0 brings x, warp 1 brings w: waiting for a stage and issuing both
     // copies takes one thread ~430 clocks, more than a narrow tile's MMAs.
@@ -233,7 +244,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
         }
       }
     }
-  } else if (warp == PROD_WARPS) {
+  } else if (warp == MMA_WARP) {
     // ------------------------------------------------------------ MMA issuer (even CTA)
     if (leader) {
       auto wait_all = [&](uint64_t* bar, uint32_t parity) {
@@ -244,35 +255,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
       bool ok = true, ready = mbar_test_wait(&full[0], 0);
       const uint32_t idesc = idesc16<T>(BM, 0) | (static_cast<uint32_t>(bn >> 3) << 17);
       const uint64_t ad0 = umma_desc_sw128(smem_u32(sA), 16, 1024), bd0 = umma_desc_sw128(smem_u32(sB), 16, 1024);
-      for (int t = cluster; t < total && ok; t += nclusters, ++local) {
-        const int buf = local & 1;
-        if (!wait_all(&tempty[buf], ((local >> 1) & 1) ^ 1u)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + buf * BN_MAX;
-        for (int kb = 0; kb < kblocks; ++kb) {
-          if (!__all_sync(0xffffffffu, ready) && !wait_all(&full[stage], phase)) {
+      for (int t = cluster; t < total && ok; t += nclusters) {
+        for (int k0 = 0; k0 < kblocks && ok; k0 += kstep, ++local) {
+          const int buf = local & 1, k1 = min(kblocks, k0 + kstep);
+          if (!wait_all(&tempty[buf], ((local >> 1) & 1) ^ 1u)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const int cur = stage;
-          if (++stage == stages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-          ready = mbar_test_wait(&full[stage], phase);
-          const uint64_t ad = ad0 + static_cast<uint64_t>((cur * A_BYTES) >> 4);
-          const uint64_t bd = bd0 + static_cast<uint64_t>((cur * b_bytes) >> 4);
+          const uint32_t d_tmem = tmem_base + buf * ACC;
+          for (int kb = k0; kb < k1; ++kb) {
+            if (!__all_sync(0xffffffffu, ready) && !wait_all(&full[stage], phase)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const int cur = stage;
+            if (++stage == stages) {
+              stage = 0;
+              phase ^= 1u;
+            }
+            ready = mbar_test_wait(&full[stage], phase);
+            const uint64_t ad = ad0 + static_cast<uint64_t>((cur * A_BYTES) >> 4);
+            const uint64_t bd = bd0 + static_cast<uint64_t>((cur * b_bytes) >> 4);
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k)
-            mma_f16_ss_pair_elect(d_tmem, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
-          mma_commit_pair_elect(&empty[cur], 0x3);
+            for (int k = 0; k < BK / 16; ++k)
+              mma_f16_ss_pair_elect(d_tmem, ad + 2 * k, bd + 2 * k, idesc, kb > k0 || k > 0 ? 1u : 0u);
+            mma_commit_pair_elect(&empty[cur], 0x3);
+          }
+          if (!ok) break;
+          mma_commit_pair_elect(&tfull[buf], 0x3);
         }
-        if (!ok) break;
-        mma_commit_pair_elect(&tfull[buf], 0x3);
       }
       if (!ok && lane == 0) {
         *abort_flag = 1;
@@ -285,7 +298,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
       while (!mbar_try_wait(drain, 0) && global_timer_ns() - t0 < kWaitLimitNs / 4) {
       }
     }
-  } else {
+  } else if (warp >= EPI_WARP0) {
     // ------------------------------------------------------------ epilogue (both CTAs)
     // A warp owns 32 rows (its TMEM lane quarter, thread = row) and every
     // second 32-column chunk of the tile: TMEM -> registers -> bias,
@@ -293,7 +306,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
     // residual, if any) -> TMA store, which clips rows and columns past the
     // end.  Two staging buffers per warp; the next chunk's residual is loaded
     // into the free one meanwhile.
-    const int quarter = warp & 3, ew = warp - PROD_WARPS - 1, half = ew >> 2;
+    const int quarter = warp & 3, ew = warp - EPI_WARP0, half = ew >> 2;
     uint8_t* ebuf = sE + ew * 2 * SUB;
     uint64_t* xb = xfull + ew * 2;
     const uint32_t tempty0 = mapa_shared(&tempty[0], 0);
@@ -302,11 +315,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
     uint32_t xphase = 0, xpending = 0;
     int local = 0, b = 0;
     bool ok = true;
-    for (int t = cluster; t < total && ok; t += nclusters, ++local) {
+    for (int t = cluster; t < total && ok; t += nclusters) {
       int m0, nt;
       pair_tile(args, t, m0, nt);
       const int r0 = m0 + 128 * static_cast<int>(cr) + quarter * 32, n0 = nt * bn_out;
-      const int buf = local & 1;
       const int nch = min(bn_out, args.N - n0 + 31) / 32;  // chunks that hold a column of the output
       const bool rows_in = r0 < args.M;
       if (resid && rows_in && half < nch && lane == 0) {
@@ -315,7 +327,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
         tma_load_2d(ebuf + b * SUB, &args.tmR, n0 + 32 * half, r0, &xb[b]);
         xpending |= 1u << b;
       }
-      bool w = mbar_wait(&tfull[buf], (local >> 1) & 1, abort_flag);
+      const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16), sum_tm = lanes + 2 * ACC;
+      bool w = true;
+      if constexpr (SUMS) {  // the accumulators before the tile's last one
+        for (int k0 = kstep; k0 < kblocks && ok; k0 += kstep, ++local) {
+          const int sb = local & 1;
+          w = mbar_wait(&tfull[sb], (local >> 1) & 1, abort_flag);
+          if (!__all_sync(0xffffffffu, w)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = half; c < nch && rows_in; c += 2)
+#pragma unroll 1
+            for (int at = 32 * c; at < bn; at += wide ? bn_out : bn) {  // SwiGLU: the chunk of gate, then of up
+              uint32_t acc[32], old[32];
+              tmem_ld32(lanes + sb * ACC + at, acc);
+              if (k0 > kstep) tmem_ld32(sum_tm + at, old);
+              tmem_ld_wait();
+              tmem_reg_fence32(acc);
+              if (k0 > kstep) {
+                tmem_reg_fence32(old);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) acc[j] = __float_as_uint(__uint_as_float(acc[j]) + __uint_as_float(old[j]));
+              }
+              tmem_st32(sum_tm + at, acc);
+            }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(tempty0 + sb * 8);
+        }
+        if (!ok) break;
+      }
+      // v += the sum's chunk at column `at`
+      auto add_sum = [&](float (&v)[32], int at) {
+        if constexpr (SUMS) {
+          uint32_t old[32];
+          tmem_ld32(sum_tm + at, old);
+          tmem_ld_wait();
+          tmem_reg_fence32(old);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(old[j]);
+        }
+      };
+      const int buf = local & 1;
+      w = mbar_wait(&tfull[buf], (local >> 1) & 1, abort_flag);
       if (!__all_sync(0xffffffffu, w)) {
         ok = false;
         break;
@@ -349,6 +407,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
         if (!ok) break;
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(acc[j]);
+        add_sum(v, 32 * c);
         if (wide) tmem_ld32(trow + bn_out + 32 * c, acc);
         if (bias) add_bias32(v, bias + col, args.N - col);
         if (wide) {
@@ -359,6 +418,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
           tmem_reg_fence32(acc);
 #pragma unroll
           for (int j = 0; j < 32; ++j) u[j] = __uint_as_float(acc[j]);
+          add_sum(u, bn_out + 32 * c);
           if (bias) add_bias32(u, bias + args.N + col, args.N - col);
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] *= u[j];
@@ -429,6 +489,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(tempty0 + buf * 8);
+      ++local;
     }
     if (lane == 0) {
       bulk_wait<0>();
@@ -449,7 +510,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // both CTAs finished with TMEM and each other's barriers
-  if (warp == PROD_WARPS) {
+  if (warp == MMA_WARP) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 512);
   }
@@ -636,10 +697,10 @@ int encode_operand(CUtensorMap* tm, const void* base, long long rows, int K, lon
 
 // Pair-tile width: the one whose waves over the SM pairs, times the tile's
 // time, finish first.
-int pair_width(int M, int cols, bool wide, int clusters) {
-  int best = 256;
+int pair_width(int M, int cols, bool wide, int most, int clusters) {
+  int best = most;
   double best_t = 1e300;
-  for (int bn = 256; bn >= 64; bn -= wide ? 64 : 32) {
+  for (int bn = most; bn >= 64; bn -= wide ? 64 : 32) {
     const long long tiles = static_cast<long long>((M + 255) / 256) * ((cols + bn - 1) / bn);
     const double t = static_cast<double>((tiles + clusters - 1) / clusters) * (bn + 48);
     if (t < best_t * 0.97) {
@@ -666,11 +727,12 @@ int launch16(void (*fn)(const A), unsigned grid, int threads, int smem, const A&
   return cudaLaunchKernelEx(&cfg, fn, args) == cudaSuccess ? QI_OK : QI_ERR_CUDA;
 }
 
-template <typename T, typename O>
+template <typename T, typename O, bool SUMS>
 int launch_pair16(const Linear16Args& a, L16Dev& d, cudaStream_t stream, int num_sms) {
   const bool wide = a.act == QI_ACT_SWIGLU;
   const int clusters = num_sms / 2;
-  d.bn = pair_width(a.M, (wide ? 2 : 1) * a.N, wide, clusters);
+  const int most = SUMS ? (wide ? pk::SUMS_BN_WIDE : pk::SUMS_BN) : pk::BN_MAX;
+  d.bn = pair_width(a.M, (wide ? 2 : 1) * a.N, wide, most, clusters);
   const int bn_out = wide ? d.bn / 2 : d.bn;
   d.tiles_m = (a.M + pk::BM - 1) / pk::BM;
   d.tiles_n = (a.N + bn_out - 1) / bn_out;
@@ -684,7 +746,7 @@ int launch_pair16(const Linear16Args& a, L16Dev& d, cudaStream_t stream, int num
       (a.residual && encode<O>(&d.tmR, a.residual, a.M, a.N, a.ldr, 32, 32, osw) != QI_OK))
     return QI_ERR_CUDA;
   static unsigned long long attr_done = 0;
-  const auto fn = linear16_pair_kernel<T, O>;
+  const auto fn = linear16_pair_kernel<T, O, SUMS>;
   if (smem_optin(reinterpret_cast<const void*>(fn), pk::SMEM_BYTES, &attr_done) != QI_OK) return QI_ERR_CUDA;
   const int tiles = d.tiles_m * d.tiles_n;
   return launch16(fn, 2u * (tiles < clusters ? tiles : clusters), pk::THREADS, pk::SMEM_BYTES, d, stream);
@@ -723,7 +785,9 @@ int launch_typed(const Linear16Args& a, cudaStream_t stream) {
   d.N = a.N;
   d.K = a.K;
   d.act = a.act;
-  return launch_pair16<T, O>(a, d, stream, device_num_sms());
+  if constexpr (sizeof(O) == 4)
+    if (a.K > pk::SUMS_MIN_K) return launch_pair16<T, O, true>(a, d, stream, device_num_sms());
+  return launch_pair16<T, O, false>(a, d, stream, device_num_sms());
 }
 
 }  // namespace

@@ -266,29 +266,37 @@ def qkv_norm_rope_i8(act_img, act_txt, w_img, w_txt, norms, pe, nb=1):
     return out
 
 
-def _on_device(t):
-    """Index of the GPU that holds t, and a guard that makes it current (None
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_workspace_bytes = {}  # sizes of a prompt_attention call -> its workspace
+
+
+def _guard(t):
+    """Index of the GPU that holds t, and a context that makes it current (None
     when it is already)."""
-    dev = t.device
-    if dev.type != "cuda":
+    index = t.get_device()
+    if index < 0:
         raise QIError("tensors must be on a GPU")
-    return dev.index, None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev.index)
+    return index, None if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 def _offsets(seq, index, what):
     """(begin pointer, end pointer, count) of a sequence argument: int32 offsets
     of packed sequences [count + 1], or a pair (begin, end) of int32 [count]."""
-    pair = isinstance(seq, (tuple, list))
-    for t in seq if pair else (seq,):
-        if t.dtype != torch.int32 or t.dim() != 1 or t.get_device() != index or not t.is_contiguous():
-            raise QIError(f"{what}: contiguous int32 offsets on the tensors' GPU")
-    if pair:
-        if len(seq) != 2 or seq[0].numel() != seq[1].numel():
-            raise QIError(f"{what}: begin and end differ in length")
-        return seq[0].data_ptr(), seq[1].data_ptr(), seq[0].numel()
-    if seq.numel() < 1:
-        raise QIError(f"{what}: one more offset than sequences")
-    return seq.data_ptr(), seq.data_ptr() + 4, seq.numel() - 1
+    if isinstance(seq, (tuple, list)):
+        if len(seq) != 2:
+            raise QIError(f"{what}: a pair (begin, end)")
+        begin, end = seq
+        n, n_end = begin.numel(), end.numel()
+        if n != n_end or end.dtype is not torch.int32 or end.dim() != 1 or end.get_device() != index or not end.is_contiguous():
+            raise QIError(f"{what}: begin and end alike, contiguous int32 on the tensors' GPU")
+        pb, pe = begin.data_ptr(), end.data_ptr()
+    else:
+        begin, n = seq, seq.numel() - 1
+        pb = begin.data_ptr()
+        pe = pb + 4
+    if n < 0 or begin.dtype is not torch.int32 or begin.dim() != 1 or begin.get_device() != index or not begin.is_contiguous():
+        raise QIError(f"{what}: contiguous int32 offsets on the tensors' GPU")
+    return pb, pe, n
 
 
 def prompt_attention(q, k, v, q_seq, k_seq, max_k, causal=True, scale=None, out=None):
@@ -302,39 +310,43 @@ def prompt_attention(q, k, v, q_seq, k_seq, max_k, causal=True, scale=None, out=
     current stream."""
     if not (q.dim() == k.dim() == v.dim() == 3):
         raise QIError("q, k, v: [rows, heads, head_dim]")
-    dt = _DT16.get(q.dtype)
-    if dt is None or k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    dt = _DT16.get(dtype)
+    if dt is None or k.dtype is not dtype or v.dtype is not dtype:
         raise QIError("q, k, v: all BF16 or all FP16")
-    index, guard = _on_device(q)
-    tq, heads, dim = q.shape
-    tk, kv, kdim = k.shape
-    if v.shape != k.shape or kdim != dim:
+    index, guard = _guard(q)
+    tq, heads, dim = qshape = q.shape
+    tk, kv, kdim = kshape = k.shape
+    if v.shape != kshape or kdim != dim:
         raise QIError("k, v: same shape, head_dim as q")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
+        out = q.new_empty(qshape)
+    elif out.shape != qshape or out.dtype is not dtype or out.get_device() != index:
         raise QIError("out: as q")
-    if not (k.get_device() == v.get_device() == out.get_device() == index):
-        raise QIError("q, k, v, out: on one GPU")
+    if not (k.get_device() == v.get_device() == index):
+        raise QIError("q, k, v: on one GPU")
     (q0, q1, q2), (k0, k1, k2), (v0, v1, v2), (o0, o1, o2) = q.stride(), k.stride(), v.stride(), out.stride()
     if not (q2 == k2 == v2 == o2 == 1):
         raise QIError("head_dim must be the contiguous dimension")
     qb, qe, nb = _offsets(q_seq, index, "q_seq")
-    kb, ke, nk = _offsets(k_seq, index, "k_seq")
+    kb, ke, nk = (qb, qe, nb) if k_seq is q_seq else _offsets(k_seq, index, "k_seq")
     if nb != nk:
         raise QIError("q_seq and k_seq: one entry per sequence")
     if guard is not None:
         with guard:
             return prompt_attention(q, k, v, q_seq, k_seq, max_k, causal, scale, out)
-    L = lib()
-    nws = L.qi_prompt_attention_workspace(heads, kv, dim, nb, tq, tk, max_k)
-    if nws:
+    sizes = (heads, kv, dim, nb, tq, tk, max_k)
+    nws = _workspace_bytes.get((sizes, index))
+    if nws is None:
+        nws = lib().qi_prompt_attention_workspace(*sizes)
         check(-nws if nws < 0 else 0)
-        ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
-    st = L.qi_prompt_attention(q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, out.data_ptr(), o0, o1, dt,
-                               heads, kv, dim, qb, qe, kb, ke, nb, tq, tk, max_k, dim ** -0.5 if scale is None else scale,
-                               1 if causal else 0, ws.data_ptr() if nws else None, nws,
-                               torch._C._cuda_getCurrentRawStream(index))
+        if len(_workspace_bytes) > 4096:
+            _workspace_bytes.clear()
+        _workspace_bytes[sizes, index] = nws
+    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
+    st = lib().qi_prompt_attention(q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, out.data_ptr(), o0, o1, dt,
+                                   heads, kv, dim, qb, qe, kb, ke, nb, tq, tk, max_k, dim ** -0.5 if scale is None else scale,
+                                   1 if causal else 0, ws.data_ptr() if nws else None, nws, _raw_stream(index))
     if st:
         check(st)
     return out
@@ -358,11 +370,10 @@ def linear_16bit(x, w, bias=None, act=ACT_NONE, gate=None, residual=None, out_dt
     N = rows // wide
     if kw != K or N * wide != rows:
         raise QIError("w [N, K]; for SwiGLU N gate rows, then N up rows")
-    index, guard = _on_device(x)
+    index, guard = _guard(x)
     if out is None:
         odt = out_dtype or (xdt if residual is None else residual.dtype)
-        out = torch.empty((M, N), dtype=odt, device=x.device) if N % 8 == 0 else torch.empty(
-            (M, -(-N // 8) * 8), dtype=odt, device=x.device)[:, :N]
+        out = x.new_empty((M, N), dtype=odt) if N % 8 == 0 else x.new_empty((M, -(-N // 8) * 8), dtype=odt)[:, :N]
     elif out.shape != (M, N) or (out_dtype is not None and out.dtype != out_dtype):
         raise QIError("out: [M, N] in out_dtype")
     odt = _DT_OUT.get(out.dtype)
@@ -401,7 +412,7 @@ def linear_16bit(x, w, bias=None, act=ACT_NONE, gate=None, residual=None, out_dt
         with guard:
             return linear_16bit(x, w, bias, act, gate, residual, None, out)
     st = lib().qi_linear_16bit(x.data_ptr(), ldx, M, K, w.data_ptr(), ldw, N, dt, bp, act, gp, rp, ldr, out.data_ptr(), ldo,
-                               odt, torch._C._cuda_getCurrentRawStream(index))
+                               odt, _raw_stream(index))
     if st:
         check(st)
     return out
