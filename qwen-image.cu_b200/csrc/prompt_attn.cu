@@ -61,7 +61,6 @@ struct alignas(64) PromptAttnDev {
   int P, T, packs;   // heads per tile row group, tokens per tile, tiles' head packs per kv head
   int items;         // work items per head pack at most: (unit of NT tiles, split of its keys) (gridDim.x)
   int splits;        // splits of a sequence's keys at most
-  int join_warps;    // warps per row of the joining kernel
   float sc;          // |scale| log2(e)
   uint32_t negate;   // scale < 0: instruction descriptor bit 13 (negate A) for Q K^T
   float* part;       // splits > 1: [splits][total_q * heads][DH] normalised partial outputs
@@ -124,86 +123,109 @@ __device__ __forceinline__ int blocks_of(int4 p, int causal) {
 }
 __device__ __forceinline__ int splits_of(int blocks, int chunk) { return max(1, (blocks + chunk - 1) / chunk); }
 
-// Key blocks per split: the smallest number that keeps all sequences' work items
-// within args.items (whole waves of CTAs) and a sequence's splits within
-// args.splits; every CTA of the call works out the same.  Called by a whole CTA;
-// leaves the first CACHED_SEQS sequences in `seqs`.
-__device__ __forceinline__ int chunk_of(const PromptAttnDev& d, int step, int* smem, int4* seqs) {
+// Which work item CTA `idx` of a head pack takes, and the key blocks per split.
+// Called by one whole warp; leaves the first CACHED_SEQS sequences in `seqs`.
+// False when there are fewer items.
+//
+// Splits: the smallest chunk of key blocks that keeps all sequences' items within
+// args.items (whole waves of CTAs) and a sequence's splits within args.splits,
+// worked out from the lengths by every CTA alike.
+// Order (BY_INDEX): a causal sequence's later units see more keys, so the units of
+// all sequences go by their index, the last first.
+template <bool BY_INDEX>
+__device__ __forceinline__ bool schedule(const PromptAttnDev& d, int step, int idx, int4* seqs, int& chunk, Place& out) {
   const PromptAttnArgs& a = d.a;
-  const int tid = threadIdx.x, nt = blockDim.x;
-  int *total = smem, *longest = smem + 1, *count = smem + 2;  // count: two, taking turns
-  if (tid < 4) smem[tid] = 0;
-  const bool split = d.splits > 1;
-  if (split) __syncthreads();
-  int u0 = 0, n0 = 0;  // this thread's first sequence
-  for (int b = tid; b < a.batch; b += nt) {
+  const int lane = threadIdx.x & 31;
+  int most = 0, most_units = 0, u0 = 0;  // u0: units of sequence `lane`
+  float work = 0.0f;
+  for (int b = lane; b < a.batch; b += 32) {
     const int4 p = sequence(a, b);
     if (b < CACHED_SEQS) seqs[b] = p;
-    if (!split) {
-      if (b + nt >= CACHED_SEQS) break;
-      continue;
-    }
     const int u = units_of(p, step), n = blocks_of(p, a.causal);
-    if (b == tid) {
-      u0 = u;
-      n0 = n;
-    }
-    // (a count that saturates only makes the first guess of the chunk smaller)
-    atomicAdd(total, static_cast<int>(min(static_cast<long long>(u) * n, 1ll << 20)));
-    atomicMax(longest, n);
+    if (b == lane) u0 = u;
+    most = max(most, n);
+    most_units = max(most_units, u);
+    work += static_cast<float>(u) * static_cast<float>(n);
   }
-  __syncthreads();
-  if (!split) return INT_MAX / 2;
-  const int most = *longest;
-  int chunk = max(max(2, (most + d.splits - 1) / d.splits), min(max(*total, 0) / d.items, most));
-  for (int turn = 0; chunk < most; turn ^= 1) {
-    int mine = tid < a.batch ? u0 * splits_of(n0, chunk) : 0;
-    for (int b = tid + nt; b < a.batch; b += nt) {
-      const int4 p = sequence(a, b);
-      mine += units_of(p, step) * splits_of(blocks_of(p, a.causal), chunk);
+  __syncwarp();
+  auto seq = [&](int b) { return b < CACHED_SEQS ? seqs[b] : sequence(a, b); };
+  auto take = [&](int4 p, int unit, int split) {
+    out.q0 = p.x;
+    out.lq = p.y;
+    out.k0 = p.z;
+    out.lk = p.w;
+    out.unit = unit;
+    out.split = split;
+  };
+  chunk = INT_MAX / 2;
+  if (BY_INDEX && d.splits == 1 && a.causal) {
+    most_units = __reduce_max_sync(0xffffffffu, most_units);
+    auto count = [&](int unit) {  // units with this index or a higher one
+      int n = max(0, u0 - unit);
+      for (int b = lane + 32; b < a.batch; b += 32) n += max(0, units_of(seq(b), step) - unit);
+      return __reduce_add_sync(0xffffffffu, n);
+    };
+    if (idx >= count(0)) return false;
+    int lo = 0, hi = most_units;  // count(lo) > idx >= count(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (count(mid) > idx)
+        lo = mid;
+      else
+        hi = mid;
     }
-    if (mine) atomicAdd(count + turn, mine);
-    __syncthreads();
-    const bool fits = count[turn] <= d.items;
-    if (tid == 0) count[turn ^ 1] = 0;
-    __syncthreads();
-    if (fits) break;
-    chunk += max(1, chunk / 8);
+    int r = idx - count(lo + 1);  // the r-th sequence that has a unit lo
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+      const int u = b0 == 0 ? u0 : (b0 + lane < a.batch ? units_of(seq(b0 + lane), step) : 0);
+      unsigned m = __ballot_sync(0xffffffffu, u > lo);
+      if (r >= __popc(m)) {
+        r -= __popc(m);
+        continue;
+      }
+      for (; r > 0; --r) m &= m - 1;
+      take(seq(b0 + __ffs(m) - 1), lo, 0);
+      return true;
+    }
+    return false;
   }
-  return chunk;
-}
-
-// Work item `u` when the sequences' items follow one another; false past the
-// last.  Called by one whole warp.
-__device__ __forceinline__ bool find_item(const PromptAttnArgs& a, int step, int chunk, int u, const int4* seqs, Place& out) {
-  const int lane = threadIdx.x & 31;
+  if (d.splits > 1) {
+    most = __reduce_max_sync(0xffffffffu, most);
+#pragma unroll
+    for (int i = 16; i > 0; i /= 2) work += __shfl_xor_sync(0xffffffffu, work, i);
+    chunk = max(max(2, (most + d.splits - 1) / d.splits), static_cast<int>(fminf(work / d.items, static_cast<float>(most))));
+    while (chunk < most) {
+      int n = 0;
+      for (int b = lane; b < a.batch; b += 32) {
+        const int4 p = seq(b);
+        n += units_of(p, step) * splits_of(blocks_of(p, a.causal), chunk);
+      }
+      if (__reduce_add_sync(0xffffffffu, n) <= d.items) break;
+      chunk += max(1, chunk / 8);
+    }
+  }
+  // the sequences' items follow one another
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
     int4 p = make_int4(0, 0, 0, 0);
     int n = 0, s = 1;
     if (b0 + lane < a.batch) {
-      p = b0 + lane < CACHED_SEQS ? seqs[b0 + lane] : sequence(a, b0 + lane);
+      p = seq(b0 + lane);
       s = splits_of(blocks_of(p, a.causal), chunk);
       n = units_of(p, step) * s;
     }
     int sum = n;  // inclusive prefix sum over the lanes
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int v = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += v;
+    for (int i = 1; i < 32; i *= 2) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, i);
+      if (lane >= i) sum += v;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, u < sum);
+    const unsigned hit = __ballot_sync(0xffffffffu, idx < sum);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      const int r = u - __shfl_sync(0xffffffffu, sum - n, src), sp = __shfl_sync(0xffffffffu, s, src);
-      out.q0 = __shfl_sync(0xffffffffu, p.x, src);
-      out.lq = __shfl_sync(0xffffffffu, p.y, src);
-      out.k0 = __shfl_sync(0xffffffffu, p.z, src);
-      out.lk = __shfl_sync(0xffffffffu, p.w, src);
-      out.unit = r / sp;
-      out.split = r % sp;
+      const int r = idx - __shfl_sync(0xffffffffu, sum - n, src), sp = __shfl_sync(0xffffffffu, s, src);
+      take(seq(b0 + src), r / sp, r % sp);
       return true;
     }
-    u -= __shfl_sync(0xffffffffu, sum, 31);
+    idx -= __shfl_sync(0xffffffffu, sum, 31);
   }
   return false;
 }
@@ -240,7 +262,7 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
   int* any_bad = const_cast<int*>(abort_flag) + 1;
   Place* place = reinterpret_cast<Place*>(any_bad + 1);
   int* found = reinterpret_cast<int*>(place + 1);
-  int* sched = found + 1;  // chunk_of's four words
+  int* chunk_slot = found + 1;
   int4* seqs = reinterpret_cast<int4*>(smem + C::OFF_X + 2048);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -271,6 +293,7 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
     tma_prefetch_desc(&args.tmQ);
     tma_prefetch_desc(&args.tmK);
     tma_prefetch_desc(&args.tmV);
+    tma_prefetch_desc(&args.tmO);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::TMEM_COLS);
@@ -280,13 +303,14 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
     for (int i = lane; i < 3 * DH; i += 32) bad[i] = INT_MAX;
   grid_dependency_wait();
   launch_dependents();
-  const int chunk = chunk_of(args, NT * args.T, sched, seqs);
-  if (warp == 0) {  // in descending order: a causal sequence's later units have more keys
+  if (warp == 0) {
     Place p = {};
-    const bool ok = find_item(a, NT * args.T, chunk, args.items - 1 - static_cast<int>(blockIdx.x), seqs, p);
+    int c;
+    const bool ok = schedule<NT == 2>(args, NT * args.T, blockIdx.x, seqs, c, p);
     if (lane == 0) {
       *place = p;
       *found = ok;
+      *chunk_slot = c;
     }
   }
   tc_fence_before();
@@ -294,6 +318,7 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const Place pl = *place;
+  const int chunk = *chunk_slot;
   const int tok0 = pl.unit * NT * args.T;  // first token of the unit in its sequence
   // key blocks [jb, je[t]) of tile t in this split; n[t] of them
   int n[NT], nkb[NT], nmax = 0;
@@ -719,27 +744,37 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
 // A CTA per token and 8 / per heads; `per` warps per head take its splits in
 // turn, four dimensions per thread, and add up in warp order.  Rows whose tile
 // had one split are final already.
+struct JoinDev {
+  void* out;
+  long long o_row, o_head;
+  const int* q_begin;
+  const int* q_end;
+  const float* part;
+  const float2* ml;
+  const int* used;
+  int batch, total_q, heads, head_dim;
+  int warps;  // per head
+};
 template <typename T, int DH>
-__global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_constant__ PromptAttnDev args) {
+__global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_constant__ JoinDev args) {
   __shared__ float4 part_o[8][32];
   __shared__ float2 part_w[8];
   grid_dependency_wait();
   launch_dependents();
-  const PromptAttnArgs& a = args.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per = args.join_warps, wi = warp % per;
+  const int per = args.warps, wi = warp % per;
   const int qrow = blockIdx.x, head = blockIdx.y * (8 / per) + warp / per;
-  const long long rows = static_cast<long long>(a.total_q) * a.heads;
-  const long long slot = static_cast<long long>(qrow) * a.heads + head;
+  const long long rows = static_cast<long long>(args.total_q) * args.heads;
+  const long long slot = static_cast<long long>(qrow) * args.heads + head;
   // read ahead of the look-up; means nothing for a row of no sequence
-  int used = head < a.heads ? args.used[slot] : 0;
+  int used = head < args.heads ? args.used[slot] : 0;
   bool found = false;
-  for (int b0 = 0; b0 < a.batch && !found; b0 += 32) {
+  for (int b0 = 0; b0 < args.batch && !found; b0 += 32) {
     bool hit = false;
-    if (b0 + lane < a.batch) hit = qrow >= a.q_begin[b0 + lane] && qrow < a.q_end[b0 + lane];
+    if (b0 + lane < args.batch) hit = qrow >= args.q_begin[b0 + lane] && qrow < args.q_end[b0 + lane];
     found = __any_sync(0xffffffffu, hit);
   }
-  const bool work = found && head < a.heads && used > 1;
+  const bool work = found && head < args.heads && used > 1;
   // this warp's splits: wi, wi + per, ...; lane i holds the i-th's (m, l)
   const int mine = work && wi < used ? (used - wi + per - 1) / per : 0;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -785,9 +820,9 @@ __global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_cons
       o = make_float4(o.x + k * v.x, o.y + k * v.y, o.z + k * v.z, o.w + k * v.w);
     }
   }
-  if (!work || 4 * lane >= a.head_dim) return;
+  if (!work || 4 * lane >= args.head_dim) return;
   const float r = total == 0.0f ? 0.0f : 1.0f / total;
-  T* out = static_cast<T*>(a.out) + qrow * a.o_row + head * a.o_head + 4 * lane;
+  T* out = static_cast<T*>(args.out) + qrow * args.o_row + head * args.o_head + 4 * lane;
   *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(o.x * r, o.y * r), pack16<T>(o.z * r, o.w * r));
 }
 
@@ -859,9 +894,11 @@ int launch_tiles(const PromptAttnDev& d, cudaStream_t stream) {
   const dim3 grid(d.items, d.a.heads / d.P);
   const int st = launch_dependent(fn, grid, C::THREADS, C::SMEM, d, stream);
   if (st != QI_OK || d.splits == 1) return st;
-  const int per_cta = 8 / d.join_warps;
-  return launch_dependent(prompt_attn_join_kernel<T, DH>, dim3(d.a.total_q, (d.a.heads + per_cta - 1) / per_cta), 256, 0, d,
-                          stream);
+  const PromptAttnArgs& a = d.a;
+  const int warps = d.splits >= 16 ? 8 : (d.splits >= 8 ? 4 : (d.splits >= 4 ? 2 : 1)), per_cta = 8 / warps;
+  const JoinDev j{a.out, a.o_row, a.o_head, a.q_begin, a.q_end, d.part, d.ml, d.used, a.batch, a.total_q, a.heads, a.head_dim,
+                  warps};
+  return launch_dependent(prompt_attn_join_kernel<T, DH>, dim3(a.total_q, (a.heads + per_cta - 1) / per_cta), 256, 0, j, stream);
 }
 
 template <typename T>
@@ -890,7 +927,6 @@ int prompt_attention_launch(const PromptAttnArgs& a, cudaStream_t stream) {
   d.packs = p.packs;
   d.items = static_cast<int>(p.items);
   d.splits = p.splits;
-  d.join_warps = p.splits >= 16 ? 8 : (p.splits >= 8 ? 4 : (p.splits >= 4 ? 2 : 1));
   d.sc = (a.scale < 0.0f ? -a.scale : a.scale) * 1.4426950408889634f;
   // scale 0: the smallest normal number does the same to finite scores (every
   // weight 1) and leaves masked ones at -inf, where 0 would make them NaN

@@ -320,7 +320,7 @@ def prompt_attention(q, k, v, q_seq, k_seq, max_k, causal=True, scale=None, out=
     if v.shape != kshape or kdim != dim:
         raise QIError("k, v: same shape, head_dim as q")
     if out is None:
-        out = q.new_empty(qshape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != qshape or out.dtype is not dtype or out.get_device() != index:
         raise QIError("out: as q")
     if not (k.get_device() == v.get_device() == index):
