@@ -30,7 +30,7 @@ struct alignas(64) L16Dev {  // pair kernel
   void* out;
   long long ldr, ldo;
   int M, N, K, act;
-  int stages;  // TMA pipeline depth
+  int stages, atoms;  // TMA pipeline depth, K blocks per stage
   int bn, tiles_m, tiles_n;
 };
 
@@ -109,7 +109,7 @@ __device__ __forceinline__ void add_bias32(float (&v)[32], const T* p, int n_val
 // ------------------------------------------------------------------ pair kernel
 namespace pk {
 constexpr int BM = 256, BN_MAX = 256;
-constexpr int A_BYTES = 128 * BK * 2;  // this CTA's 128 rows of x
+constexpr int A_BLOCK = 128 * BK * 2;  // this CTA's 128 rows of x, one K block
 constexpr int MMA_WARP = 2, EPI_WARP0 = 3, EPI_WARPS = 8;  // warps 0 and 1 produce
 constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS);
 // Long sums (FP32 outputs, K > 4096).  The tensor cores round every addition to
@@ -148,9 +148,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
   constexpr int ACC = SUMS ? SUMS_BN : BN_MAX;  // TMEM columns of an accumulator; SUMS: the sum at 2 ACC
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int stages = args.stages, b_bytes = args.bn / 2 * BK * 2;  // b: this CTA's half of the tile's w rows
+  const int stages = args.stages, atoms = args.atoms;
+  const int b_block = args.bn / 2 * BK * 2;  // this CTA's half of the tile's w rows, one K block
+  const int a_bytes = atoms * A_BLOCK, b_bytes = atoms * b_block;
   uint8_t* sA = smem;
-  uint8_t* sB = smem + stages * A_BYTES;
+  uint8_t* sB = smem + stages * a_bytes;
   uint8_t* sE = sB + stages * b_bytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(sE + EPI_WARPS * 2 * SUB);
   uint64_t* empty = full + MAX_STAGES;
@@ -207,7 +209,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
     // copies takes one thread ~430 clocks, more than a narrow tile's MMAs.
     if (lane == 0) {
       const uint32_t full0 = mapa_shared(&full[0], 0);  // the even CTA's stage barriers
-      const uint32_t stage_tx = 2 * (A_BYTES + b_bytes);  // both CTAs' bytes
+      const uint32_t stage_tx = 2 * (a_bytes + b_bytes);  // both CTAs' bytes
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -220,14 +222,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
         const int row = warp == 0 ? m0 + 128 * static_cast<int>(cr) : wrow;
         const CUtensorMap* tm = warp == 0 ? &args.tmX : &args.tmW;
         uint8_t* dst = warp == 0 ? sA : sB;
-        const int bytes = warp == 0 ? A_BYTES : b_bytes;
-        for (int kb = 0; kb < kblocks; ++kb) {
+        const int block = warp == 0 ? A_BLOCK : b_block;
+        for (int kb = 0; kb < kblocks; kb += atoms) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag)) {
             ok = false;
             break;
           }
           if (leader && warp == 0) mbar_expect_tx(&full[stage], stage_tx);
-          tma_load_2d_pair(dst + stage * bytes, tm, kb * BK, row, full0 + stage * 8);
+          uint8_t* to = dst + stage * atoms * block;
+          tma_load_2d_pair(to, tm, kb * BK, row, full0 + stage * 8);
+          if (atoms == 2) tma_load_2d_pair(to + block, tm, (kb + 1) * BK, row, full0 + stage * 8);  // past K: zeros
           if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
@@ -264,7 +268,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
           }
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + buf * ACC;
-          for (int kb = k0; kb < k1; ++kb) {
+          for (int kb = k0; kb < k1; kb += atoms) {
             if (!__all_sync(0xffffffffu, ready) && !wait_all(&full[stage], phase)) {
               ok = false;
               break;
@@ -276,11 +280,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
               phase ^= 1u;
             }
             ready = mbar_test_wait(&full[stage], phase);
-            const uint64_t ad = ad0 + static_cast<uint64_t>((cur * A_BYTES) >> 4);
-            const uint64_t bd = bd0 + static_cast<uint64_t>((cur * b_bytes) >> 4);
+            uint64_t ad = ad0 + static_cast<uint64_t>((cur * a_bytes) >> 4);
+            uint64_t bd = bd0 + static_cast<uint64_t>((cur * b_bytes) >> 4);
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k)
               mma_f16_ss_pair_elect(d_tmem, ad + 2 * k, bd + 2 * k, idesc, kb > k0 || k > 0 ? 1u : 0u);
+            if (atoms == 2) {
+              ad += A_BLOCK >> 4;
+              bd += static_cast<uint64_t>(b_block >> 4);
+#pragma unroll
+              for (int k = 0; k < BK / 16; ++k) mma_f16_ss_pair_elect(d_tmem, ad + 2 * k, bd + 2 * k, idesc, 1u);
+            }
             mma_commit_pair_elect(&empty[cur], 0x3);
           }
           if (!ok) break;
@@ -737,7 +747,12 @@ int launch_pair16(const Linear16Args& a, L16Dev& d, cudaStream_t stream, int num
   d.tiles_m = (a.M + pk::BM - 1) / pk::BM;
   d.tiles_n = (a.N + bn_out - 1) / bn_out;
   if (static_cast<long long>(d.tiles_m) * d.tiles_n > 0x7fffffff) return QI_ERR_UNSUPPORTED;
-  d.stages = pk::stage_room<O>() / (pk::A_BYTES + d.bn / 2 * BK * 2);
+  // Two K blocks per stage for narrow tiles, where a stage's waits and barriers
+  // cost more than one block of MMAs (N 4608, K 3584, one / two: 96 rows 17.9 /
+  // 16.0 us, 512 rows 19.4 / 17.9); wider tiles need the stages (700 rows x 3584
+  // x 14336, 160 wide: 62 / 66 us)
+  d.atoms = d.bn <= 128 ? 2 : 1;
+  d.stages = pk::stage_room<O>() / (d.atoms * (pk::A_BLOCK + d.bn / 2 * BK * 2));
   if (d.stages > pk::MAX_STAGES) d.stages = pk::MAX_STAGES;
   const CUtensorMapSwizzle osw = sizeof(O) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   if (encode_operand<T>(&d.tmX, a.x, a.M, a.K, a.ldx, 128) != QI_OK ||
