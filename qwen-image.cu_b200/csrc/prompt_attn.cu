@@ -895,7 +895,12 @@ int launch_tiles(const PromptAttnDev& d, cudaStream_t stream) {
   const int st = launch_dependent(fn, grid, C::THREADS, C::SMEM, d, stream);
   if (st != QI_OK || d.splits == 1) return st;
   const PromptAttnArgs& a = d.a;
-  const int warps = d.splits >= 16 ? 8 : (d.splits >= 8 ? 4 : (d.splits >= 4 ? 2 : 1)), per_cta = 8 / warps;
+  // warps per head: several while there are few rows (a row's splits are a chain
+  // of loads otherwise), one when the rows alone fill the device
+  const long long rows = static_cast<long long>(a.total_q) * a.heads;
+  int warps = d.splits >= 16 ? 8 : (d.splits >= 8 ? 4 : (d.splits >= 4 ? 2 : 1));
+  while (warps > 1 && rows * warps > 8192) warps /= 2;
+  const int per_cta = 8 / warps;
   const JoinDev j{a.out, a.o_row, a.o_head, a.q_begin, a.q_end, d.part, d.ml, d.used, a.batch, a.total_q, a.heads, a.head_dim,
                   warps};
   return launch_dependent(prompt_attn_join_kernel<T, DH>, dim3(a.total_q, (a.heads + per_cta - 1) / per_cta), 256, 0, j, stream);
