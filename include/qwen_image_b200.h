@@ -190,8 +190,9 @@ int qi_qkv_norm_rope_i8(const int8_t* act_img, const float* act_img_scales, cons
  * materialised softmax, cuda_kernels.cu:1162-1240): 16-bit floating point in
  * and out, FP32 sums, no context, no device allocation, no state kept between
  * calls.  Concurrent calls on any streams are independent, and both can be
- * captured into a CUDA graph.  The current device must be the one that holds
- * the buffers.                                                              */
+ * captured into a CUDA graph (after a first call on the device, which does
+ * one-time set-up).  The current device must be the one that holds the
+ * buffers.  Rows, columns and K up to 2^30 (QI_ERR_UNSUPPORTED).            */
 enum { QI_DT_BF16 = 0, QI_DT_F16 = 1, QI_DT_F32 = 2 };
 enum { QI_ACT_NONE = 0, QI_ACT_GELU = 1, QI_ACT_SILU = 2, QI_ACT_SWIGLU = 3 };
 
@@ -208,7 +209,9 @@ enum { QI_ACT_NONE = 0, QI_ACT_GELU = 1, QI_ACT_SILU = 2, QI_ACT_SWIGLU = 3 };
  * against a cache.  A query that sees no key gives zeros.  Rows of out in no
  * query range are not written.  What rows of k and v outside a sequence's
  * range hold, or at positions a query does not see, does not reach that
- * query's result, NaN and infinities included.
+ * query's result, NaN and infinities included.  out may be q itself (same
+ * pointer and strides); otherwise it shares no element with q, k or v
+ * (QI_ERR_ARG).
  * Element (row, head, d) of x is x[row * x_row + head * x_head + d]; strides
  * are in elements, positive and multiples of 8, pointers 16-byte aligned
  * (QI_ERR_ALIGN); rows and heads of out must not overlap one another.  total_q and

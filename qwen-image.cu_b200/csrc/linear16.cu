@@ -734,7 +734,9 @@ int launch16(void (*fn)(const A), unsigned grid, int threads, int smem, const A&
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fn, args) == cudaSuccess ? QI_OK : QI_ERR_CUDA;
+  if (cudaLaunchKernelEx(&cfg, fn, args) == cudaSuccess) return QI_OK;
+  cudaGetLastError();  // reported by status, not left for the caller's next check
+  return QI_ERR_CUDA;
 }
 
 template <typename T, typename O, bool SUMS>
@@ -746,7 +748,7 @@ int launch_pair16(const Linear16Args& a, L16Dev& d, cudaStream_t stream, int num
   const int bn_out = wide ? d.bn / 2 : d.bn;
   d.tiles_m = (a.M + pk::BM - 1) / pk::BM;
   d.tiles_n = (a.N + bn_out - 1) / bn_out;
-  if (static_cast<long long>(d.tiles_m) * d.tiles_n > 0x7fffffff) return QI_ERR_UNSUPPORTED;
+  if (static_cast<long long>(d.tiles_m) * d.tiles_n > 0x3fffffff) return QI_ERR_UNSUPPORTED;
   // Two K blocks per stage for narrow tiles, where a stage's waits and barriers
   // cost more than one block of MMAs (N 4608, K 3584, one / two: 96 rows 17.9 /
   // 16.0 us, 512 rows 19.4 / 17.9); wider tiles need the stages (700 rows x 3584

@@ -302,7 +302,6 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
   if (warp == 2)
     for (int i = lane; i < 3 * DH; i += 32) bad[i] = INT_MAX;
   grid_dependency_wait();
-  launch_dependents();
   if (warp == 0) {
     Place p = {};
     int c;
@@ -316,6 +315,7 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  launch_dependents();  // after the allocation: a dependent CTA on this SM gets what is left of TMEM
   const uint32_t tmem = *tmem_slot;
   const Place pl = *place;
   const int chunk = *chunk_slot;
@@ -881,7 +881,9 @@ int launch_dependent(void (*fn)(const A), dim3 grid, int threads, int smem, cons
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fn, args) == cudaSuccess ? QI_OK : QI_ERR_CUDA;
+  if (cudaLaunchKernelEx(&cfg, fn, args) == cudaSuccess) return QI_OK;
+  cudaGetLastError();  // reported by status, not left for the caller's next check
+  return QI_ERR_CUDA;
 }
 
 template <typename T, int DH, int NT>

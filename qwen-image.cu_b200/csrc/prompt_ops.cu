@@ -28,10 +28,35 @@ int check_stride(long long stride, long long n) {
   return stride % 8 ? QI_ERR_ALIGN : QI_OK;
 }
 
+// [rows][heads][dim] elements of 2 bytes at p, stepping row and head elements.
+struct Strided {
+  const void* p;
+  long long rows, heads, dim, row, head;
+  long long bytes() const {
+    return rows > 0 ? 2 * ((rows > 1 ? (rows - 1) * row : 0) + (heads > 1 ? (heads - 1) * head : 0) + dim) : 0;
+  }
+};
+
+// Whether two such tensors may share an element.  Apart: disjoint byte ranges,
+// or (views into the rows of one buffer) the same row stride, with each row's
+// heads of the one clear of the other's.
+bool may_share(const Strided& a, const Strided& b) {
+  if (!overlap(a.p, a.bytes(), b.p, b.bytes())) return false;
+  if (a.rows <= 1 || b.rows <= 1 || a.row != b.row) return true;
+  const long long fa = (a.heads > 1 ? (a.heads - 1) * a.head : 0) + a.dim, fb = (b.heads > 1 ? (b.heads - 1) * b.head : 0) + b.dim;
+  const long long diff = (static_cast<long long>(reinterpret_cast<uintptr_t>(b.p)) -
+                          static_cast<long long>(reinterpret_cast<uintptr_t>(a.p))) / 2;
+  const long long d = ((diff % a.row) + a.row) % a.row;  // where b's heads start in a's rows
+  return d < fa || d + fb > a.row;
+}
+
+constexpr int kMaxExtent = 1 << 30;  // rows, columns: index arithmetic in int with room for a tile
+
 int check_sizes(int heads, int kv_heads, int head_dim, int batch, int total_q, int total_k, int max_k) {
   if (heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1) return QI_ERR_ARG;
   if (batch < 0 || total_q < 0 || total_k < 0 || max_k < 0) return QI_ERR_ARG;
   if (head_dim % 8 || head_dim > 128 || heads > 65535) return QI_ERR_UNSUPPORTED;
+  if (total_q > kMaxExtent || total_k > kMaxExtent) return QI_ERR_UNSUPPORTED;
   return QI_OK;
 }
 }  // namespace
@@ -69,6 +94,10 @@ extern "C" int qi_prompt_attention(const void* q, long long q_row, long long q_h
   if (heads > 1 && total_q > 1 && o_row < row_span && o_head < head_span) return QI_ERR_ARG;
   if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out)) return QI_ERR_ALIGN;
   if (workspace && misaligned(workspace)) return QI_ERR_ALIGN;
+  const Strided sq{q, total_q, heads, head_dim, q_row, q_head}, so{out, total_q, heads, head_dim, o_row, o_head};
+  const Strided sk{k, total_k, kv_heads, head_dim, k_row, k_head}, sv{v, total_k, kv_heads, head_dim, v_row, v_head};
+  const bool in_place = out == q && (total_q <= 1 || o_row == q_row) && (heads <= 1 || o_head == q_head);
+  if ((!in_place && may_share(so, sq)) || may_share(so, sk) || may_share(so, sv)) return QI_ERR_ARG;
   const long long need = prompt_attention_workspace(heads, kv_heads, head_dim, batch, total_q, max_k);
   if (need > 0 && (!workspace || workspace_bytes < need)) return QI_ERR_ARG;
   PromptAttnArgs a{q, k, v, out, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, dtype, heads, kv_heads,
@@ -85,7 +114,7 @@ extern "C" int qi_linear_16bit(const void* x, long long ldx, int M, int K, const
   if (act < QI_ACT_NONE || act > QI_ACT_SWIGLU) return QI_ERR_ARG;
   if (M < 0 || N < 1 || K < 1) return QI_ERR_ARG;
   const long long wide = act == QI_ACT_SWIGLU ? 2 : 1;
-  if (wide * N > 0x7fffffffll) return QI_ERR_UNSUPPORTED;
+  if (M > kMaxExtent || K > kMaxExtent || wide * N > kMaxExtent) return QI_ERR_UNSUPPORTED;
   if (M == 0) return QI_OK;
   if (!x || !w || !out) return QI_ERR_ARG;
   const long long lim = 1ll << 38;

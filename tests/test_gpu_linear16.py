@@ -222,3 +222,24 @@ def test_binding_refuses():
     buf = rand((8, 72), 40, BF)
     with pytest.raises(Q.QIError):  # residual shifted against out
         Q.linear_16bit(x, w, residual=buf[:, :64], out=buf[:, 8:])
+
+
+@pytest.mark.parametrize("M", [3, 130, 600])
+@pytest.mark.parametrize("act", [Q.ACT_NONE, Q.ACT_GELU, Q.ACT_SWIGLU])
+def test_long_sums_in_fp32(M, act):
+    """K past the length from which FP32 outputs add their accumulators up in
+    parts of 2048: the error stays that of such a part.  Of n = 2048 / 16 = 128
+    additions that round towards zero, on a sum that grows as the square root of
+    their number, each loses 2^-24 of the sum on average: 2/3 n 2^-24 = 5.1e-6 of
+    the part, so of the whole (1 / 7 of what K = 14336 in one sum loses).  GELU
+    has a slope of at most 1.13, SwiGLU two such factors, one under a slope of 1.1."""
+    bound = {Q.ACT_NONE: 5.1e-6, Q.ACT_GELU: 5.8e-6, Q.ACT_SWIGLU: 1.1e-5}[act]
+    wide = 2 if act == Q.ACT_SWIGLU else 1
+    for K in (4104, 14336):
+        x, w = operands(M, 328, K, BF, wide, seed=60 + M)
+        got = check(x, w, F32, act=act)
+        want, _ = reference(x, w, None, act, None, None, F32)
+        assert float((got.double() - want).norm() / want.norm()) <= bound
+        # in place, with everything in the epilogue
+        stream = rand((M, 328), 61)
+        check(x, w, F32, act=act, bias=rand((wide * 328,), 62, BF), gate=rand((328,), 63), residual=stream, out=stream)

@@ -307,3 +307,47 @@ def test_binding_refuses():
             Q.prompt_attention(*args, 6)
     with pytest.raises(Q.QIError):
         Q.prompt_attention(q, k, v, cu, cu, 6, out=q[:1].expand(10, 4, 64))
+
+
+@pytest.mark.parametrize("lq", ["same", "one"])
+def test_many_sequences(lq):
+    """More sequences than a CTA keeps in shared memory, short and long ones mixed."""
+    lk = [(37 * i) % 90 for i in range(300)] + [700, 1, 0, 300]
+    lq = lk if lq == "same" else [1] * len(lk)
+    cq, ck = offsets(lq), offsets(lk)
+    q, k, v = rand((sum(lq), 8, 128), 50, BF), rand((sum(lk), 2, 128), 51, BF), rand((sum(lk), 2, 128), 52, BF)
+    check(q, k, v, cq, ck, max(lk))
+
+
+@pytest.mark.parametrize("lens,lk", [([200, 31, 128], None), ([1, 1, 3], [2000, 700, 5])])
+def test_output_over_the_queries(lens, lk):
+    """out = q: the same results, also as views into one buffer of q, k and v rows."""
+    lk = lk or lens
+    cq, ck = offsets(lens), offsets(lk)
+    q, k, v = rand((sum(lens), 8, 128), 53, BF), rand((sum(lk), 2, 128), 54, BF), rand((sum(lk), 2, 128), 55, BF)
+    want = Q.prompt_attention(q, k, v, cq, ck, max(lk))
+    mine = q.clone()
+    assert Q.prompt_attention(mine, k, v, cq, ck, max(lk), out=mine).data_ptr() == mine.data_ptr()
+    assert torch.equal(mine, want)
+    if lk == lens:
+        rows = torch.cat([q, k, v], 1)
+        Q.prompt_attention(rows[:, :8], rows[:, 8:10], rows[:, 10:], cq, ck, max(lk), out=rows[:, :8])
+        assert torch.equal(rows[:, :8], want) and torch.equal(rows[:, 8:10], k) and torch.equal(rows[:, 10:], v)
+
+
+def test_output_over_keys_or_values_is_refused():
+    rows = rand((40, 12, 64), 56, BF)
+    q, k, v = rows[:, :4], rows[:, 4:8], rows[:, 8:]
+    cu = offsets([40])
+    for out in (k, v, rows[:, 2:6]):
+        with pytest.raises(Q.QIError):
+            Q.prompt_attention(q, k, v, cu, cu, 40, out=out)
+
+
+def test_two_tiles_with_split_keys():
+    """Enough queries for two-tile CTAs, few enough to split the keys."""
+    lq, lk = [900, 700], [4000, 700]
+    cq, ck = offsets(lq), offsets(lk)
+    q, k, v = rand((1600, 14, 128), 57, BF), rand((4700, 1, 128), 58, BF), rand((4700, 1, 128), 59, BF)
+    check(q, k, v, cq, ck, 4000)
+    check(q, k, v, cq, ck, 4000, causal=False)

@@ -94,3 +94,24 @@ def test_binding_refuses_cpu_tensors():
     with pytest.raises(Q.QIError):
         Q.prompt_attention(x.view(4, 1, 64), x.view(4, 1, 64), x.view(4, 1, 64), cu, cu, 4)
     assert ctypes.sizeof(ctypes.c_longlong) == 8
+
+
+# stand-ins far apart, so that only what is changed can overlap
+FAR = dict(q=1 << 20, k=1 << 24, v=1 << 25, out=1 << 26)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(q=0), ARG), (dict(k=0), ARG), (dict(v=0), ARG), (dict(out=0), ARG), (dict(qe=0), ARG), (dict(kb=0), ARG),
+    (dict(out=1 << 24), ARG), (dict(out=1 << 25), ARG), (dict(out=(1 << 20) + 16), ARG),  # over k, v, part of q
+    (dict(out=1 << 20, o_row=1024), ARG),  # q's memory, other strides
+    (dict(q_row=1024, k_row=1024, v_row=1024, k=(1 << 20) + 1024, v=(1 << 20) + 1536, out=(1 << 20) + 512, o_row=1024), ARG),
+    (dict(total_q=(1 << 30) + 1), UNSUPPORTED), (dict(total_k=(1 << 30) + 1), UNSUPPORTED),
+])
+def test_attention_refuses_overlaps_and_extents(kw, status):
+    assert attention(**{**FAR, **kw}) == status
+
+
+@pytest.mark.parametrize("kw", [dict(M=(1 << 30) + 1), dict(K=(1 << 30) + 8, ldx=(1 << 30) + 8, ldw=(1 << 30) + 8),
+                                dict(N=(1 << 30) + 8, ldo=(1 << 30) + 8)])
+def test_linear_refuses_extents(kw):
+    assert linear(**kw) == UNSUPPORTED
