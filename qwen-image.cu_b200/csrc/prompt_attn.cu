@@ -136,13 +136,16 @@ template <bool BY_INDEX>
 __device__ __forceinline__ bool schedule(const PromptAttnDev& d, int step, int idx, int4* seqs, int& chunk, Place& out) {
   const PromptAttnArgs& a = d.a;
   const int lane = threadIdx.x & 31;
-  int most = 0, most_units = 0, u0 = 0;  // u0: units of sequence `lane`
+  int most = 0, most_units = 0, u0 = 0, n0 = 0;  // u0, n0: units and blocks of sequence `lane`
   float work = 0.0f;
   for (int b = lane; b < a.batch; b += 32) {
     const int4 p = sequence(a, b);
     if (b < CACHED_SEQS) seqs[b] = p;
     const int u = units_of(p, step), n = blocks_of(p, a.causal);
-    if (b == lane) u0 = u;
+    if (b == lane) {
+      u0 = u;
+      n0 = n;
+    }
     most = max(most, n);
     most_units = max(most_units, u);
     work += static_cast<float>(u) * static_cast<float>(n);
@@ -192,10 +195,10 @@ __device__ __forceinline__ bool schedule(const PromptAttnDev& d, int step, int i
     most = __reduce_max_sync(0xffffffffu, most);
 #pragma unroll
     for (int i = 16; i > 0; i /= 2) work += __shfl_xor_sync(0xffffffffu, work, i);
-    chunk = max(max(2, (most + d.splits - 1) / d.splits), static_cast<int>(fminf(work / d.items, static_cast<float>(most))));
+    chunk = max(max(2, (most + d.splits - 1) / d.splits), static_cast<int>(ceilf(fminf(work / d.items, static_cast<float>(most)))));
     while (chunk < most) {
-      int n = 0;
-      for (int b = lane; b < a.batch; b += 32) {
+      int n = u0 * splits_of(n0, chunk);
+      for (int b = lane + 32; b < a.batch; b += 32) {
         const int4 p = seq(b);
         n += units_of(p, step) * splits_of(blocks_of(p, a.causal), chunk);
       }
@@ -205,12 +208,17 @@ __device__ __forceinline__ bool schedule(const PromptAttnDev& d, int step, int i
   }
   // the sequences' items follow one another
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    int4 p = make_int4(0, 0, 0, 0);
-    int n = 0, s = 1;
-    if (b0 + lane < a.batch) {
-      p = seq(b0 + lane);
-      s = splits_of(blocks_of(p, a.causal), chunk);
-      n = units_of(p, step) * s;
+    int n = u0, s = n0;
+    if (b0 > 0) {
+      const int4 p = b0 + lane < a.batch ? seq(b0 + lane) : make_int4(0, 0, 0, 0);
+      n = units_of(p, step);
+      s = blocks_of(p, a.causal);
+    }
+    if (d.splits > 1) {
+      s = splits_of(s, chunk);
+      n *= s;
+    } else {
+      s = 1;
     }
     int sum = n;  // inclusive prefix sum over the lanes
 #pragma unroll
@@ -628,7 +636,9 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
     if (ok && my_n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_final[t], 0, abort_flag));
     // splits of this tile that hold keys; with one the output is final
     const int used = splits_of(my_nkb, chunk);
-    const bool all_rows = used == 1 && pl.split == 0 && *found && tok0 + (t + 1) * args.T <= pl.lq;
+    // (two tiles: one-tile CTAs end sooner without a bulk store's round trip.
+    // Packed prompts 76 / 83 us with / without it, chunks behind caches 42 / 39)
+    const bool all_rows = NT == 2 && used == 1 && pl.split == 0 && *found && tok0 + (t + 1) * args.T <= pl.lq;
     auto tile_sync = [&]() {  // the tile's four warps
       if (t == 0)
         asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -753,10 +763,11 @@ struct JoinDev {
   const float2* ml;
   const int* used;
   int batch, total_q, heads, head_dim;
-  int warps;  // per head
+  int warps, splits;  // warps per head; splits the workspace holds
 };
 template <typename T, int DH>
 __global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_constant__ JoinDev args) {
+  constexpr int AHEAD = 6;
   __shared__ float4 part_o[8][32];
   __shared__ float2 part_w[8];
   grid_dependency_wait();
@@ -766,8 +777,18 @@ __global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_cons
   const int qrow = blockIdx.x, head = blockIdx.y * (8 / per) + warp / per;
   const long long rows = static_cast<long long>(args.total_q) * args.heads;
   const long long slot = static_cast<long long>(qrow) * args.heads + head;
-  // read ahead of the look-up; means nothing for a row of no sequence
-  int used = head < args.heads ? args.used[slot] : 0;
+  // Read ahead of the look-up, to have one round trip to memory instead of
+  // three: the row's split count, this warp's first (m, l) and, with few rows
+  // (per > 1), partial outputs, all inside the workspace; what is past the row's splits, or belongs
+  // to no sequence, means nothing and is not used
+  const int used = head < args.heads ? args.used[slot] : 0;
+  float2 ml0 = make_float2(-INFINITY, 0.0f);
+  if (head < args.heads && wi + lane * per < args.splits) ml0 = args.ml[(wi + static_cast<long long>(lane) * per) * rows + slot];
+  float4 v0[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (per > 1 && head < args.heads && wi + i * per < args.splits && 4 * lane < DH)
+      v0[i] = *reinterpret_cast<const float4*>(args.part + ((wi + static_cast<long long>(i) * per) * rows + slot) * DH + 4 * lane);
   bool found = false;
   for (int b0 = 0; b0 < args.batch && !found; b0 += 32) {
     bool hit = false;
@@ -782,7 +803,7 @@ __global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_cons
   for (int i0 = 0; i0 < mine; i0 += 32) {
     const long long s = wi + static_cast<long long>(i0 + lane) * per;
     float2 ml = make_float2(-INFINITY, 0.0f);
-    if (i0 + lane < mine) ml = args.ml[s * rows + slot];
+    if (i0 + lane < mine) ml = i0 == 0 ? ml0 : args.ml[s * rows + slot];
     float t = ml.y == 0.0f ? -INFINITY : ml.x;  // l = 0: this part saw nothing
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
@@ -792,8 +813,16 @@ __global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_cons
     total *= keep;
     o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
     const float w_lane = ml.y == 0.0f ? 0.0f : ml.y * ex2(ml.x - top);
+    const int ahead = per > 1 && i0 == 0 ? min(mine, AHEAD) : 0;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const float w = __shfl_sync(0xffffffffu, w_lane, i);
+      if (i >= ahead || w == 0.0f || 4 * lane >= DH) continue;
+      total += w;
+      o = make_float4(o.x + w * v0[i].x, o.y + w * v0[i].y, o.z + w * v0[i].z, o.w + w * v0[i].w);
+    }
 #pragma unroll 4
-    for (int i = 0; i < min(mine - i0, 32); ++i) {
+    for (int i = ahead; i < min(mine - i0, 32); ++i) {
       const float w = __shfl_sync(0xffffffffu, w_lane, i);
       if (w == 0.0f || 4 * lane >= DH) continue;
       const float4 v = *reinterpret_cast<const float4*>(
@@ -904,7 +933,7 @@ int launch_tiles(const PromptAttnDev& d, cudaStream_t stream) {
   while (warps > 1 && rows * warps > 8192) warps /= 2;
   const int per_cta = 8 / warps;
   const JoinDev j{a.out, a.o_row, a.o_head, a.q_begin, a.q_end, d.part, d.ml, d.used, a.batch, a.total_q, a.heads, a.head_dim,
-                  warps};
+                  warps, d.splits};
   return launch_dependent(prompt_attn_join_kernel<T, DH>, dim3(a.total_q, (a.heads + per_cta - 1) / per_cta), 256, 0, j, stream);
 }
 
