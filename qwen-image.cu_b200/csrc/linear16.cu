@@ -389,7 +389,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
         break;
       }
       tc_fence_after();
-      const uint32_t trow = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN_MAX;
+      const uint32_t trow = lanes + buf * ACC;
       for (int c = half; c < nch && rows_in; c += 2, b ^= 1) {
         const int col = n0 + 32 * c;
         uint8_t* sbuf = ebuf + b * SUB;

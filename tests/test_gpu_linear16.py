@@ -243,3 +243,17 @@ def test_long_sums_in_fp32(M, act):
         # in place, with everything in the epilogue
         stream = rand((M, 328), 61)
         check(x, w, F32, act=act, bias=rand((wide * 328,), 62, BF), gate=rand((328,), 63), residual=stream, out=stream)
+
+
+@pytest.mark.parametrize("M,N", [(130, 328), (2100, 4104)])
+@pytest.mark.parametrize("K", [4160, 6200, 8192, 12288, 16384])
+@pytest.mark.parametrize("act", [Q.ACT_NONE, Q.ACT_SWIGLU])
+def test_long_sums_of_even_and_odd_parts(M, N, K, act):
+    """2 to 8 parts of 2048, in the first tile of a CTA pair and in later ones:
+    a tile's last part may be in either accumulator.  Bounds as above."""
+    wide = 2 if act == Q.ACT_SWIGLU else 1
+    x, w = operands(M, N, K, BF, wide, seed=70 + K)
+    stream = rand((M, N), 71)
+    got = check(x, w, F32, act=act, residual=stream)
+    want, _ = reference(x, w, None, act, None, stream, F32)
+    assert float((got.double() - want).norm() / want.norm()) <= (1.1e-5 if wide == 2 else 5.1e-6)
