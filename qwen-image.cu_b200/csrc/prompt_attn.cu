@@ -779,9 +779,11 @@ __global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_cons
   const long long slot = static_cast<long long>(qrow) * args.heads + head;
   // Read ahead of the look-up, to have one round trip to memory instead of
   // three: the row's split count, this warp's first (m, l) and, with few rows
-  // (per > 1), partial outputs, all inside the workspace; what is past the row's splits, or belongs
-  // to no sequence, means nothing and is not used
-  const int used = head < args.heads ? args.used[slot] : 0;
+  // (per > 1), partial outputs, all inside the workspace; what is past the
+  // row's splits, or belongs to no sequence, means nothing and is not used.
+  // The count is bounded: query ranges that overlap can ask for more items than
+  // the grid has, and rows of those that are left out have no count
+  const int used = head < args.heads ? min(args.used[slot], args.splits) : 0;
   float2 ml0 = make_float2(-INFINITY, 0.0f);
   if (head < args.heads && wi + lane * per < args.splits) ml0 = args.ml[(wi + static_cast<long long>(lane) * per) * rows + slot];
   float4 v0[AHEAD];

@@ -351,3 +351,25 @@ def test_two_tiles_with_split_keys():
     q, k, v = rand((1600, 14, 128), 57, BF), rand((4700, 1, 128), 58, BF), rand((4700, 1, 128), 59, BF)
     check(q, k, v, cq, ck, 4000)
     check(q, k, v, cq, ck, 4000, causal=False)
+
+
+def test_overlapping_query_ranges_read_nothing_outside_the_workspace():
+    """Not allowed, and the rows' results mean nothing, but the lengths live on
+    the device: a call whose ranges ask for more tiles than there are CTAs joins
+    rows that no CTA has made, whatever the workspace held before."""
+    heads, kv, dim, batch, tq, lk = 28, 4, 128, 64, 100, 4096
+    q, k, v = rand((tq, heads, dim), 1, BF), rand((lk, kv, dim), 2, BF), rand((lk, kv, dim), 3, BF)
+    begin = torch.tensor([0] * (batch - 1) + [90], dtype=torch.int32, device="cuda")
+    end = torch.tensor([90] * (batch - 1) + [tq], dtype=torch.int32, device="cuda")
+    ks, ke = torch.zeros(batch, dtype=torch.int32, device="cuda"), torch.full((batch,), lk, dtype=torch.int32, device="cuda")
+    n = Q.lib().qi_prompt_attention_workspace(heads, kv, dim, batch, tq, lk, lk)
+    assert n > 0
+    ws = torch.full((n,), 0x7F, dtype=torch.uint8, device="cuda")
+    out = torch.zeros_like(q)
+    st = Q.lib().qi_prompt_attention(
+        q.data_ptr(), heads * dim, dim, k.data_ptr(), kv * dim, dim, v.data_ptr(), kv * dim, dim, out.data_ptr(), heads * dim, dim,
+        Q.DT_BF16, heads, kv, dim, begin.data_ptr(), end.data_ptr(), ks.data_ptr(), ke.data_ptr(), batch, tq, lk, lk,
+        dim**-0.5, 0, ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream)
+    assert st == 0
+    torch.cuda.synchronize()
+    Q.prompt_ops_check()
