@@ -633,7 +633,9 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
       f2unpack(f2add(f2add(sum2[0], sum2[1]), f2add(sum2[2], sum2[3])), a0, a1);
       l = l * alpha + (a0 + a1);
     }
-    if (ok && my_n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_final[t], 0, abort_flag));
+    // a tile without keys stages zeros where its Q may still be on its way, for
+    // the other tile's sake (the producer brings both tiles' Q)
+    if (ok && nmax > 0) ok = __all_sync(0xffffffffu, mbar_wait(my_n > 0 ? &o_final[t] : q_full, 0, abort_flag));
     // splits of this tile that hold keys; with one the output is final
     const int used = splits_of(my_nkb, chunk);
     // (two tiles: one-tile CTAs end sooner without a bulk store's round trip.

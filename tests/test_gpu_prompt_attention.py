@@ -353,6 +353,19 @@ def test_two_tiles_with_split_keys():
     check(q, k, v, cq, ck, 4000, causal=False)
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(64, 8, 128), (20, 4, 64), (6, 6, 128)])
+def test_tile_without_keys_next_to_one_with_keys(heads, kv, dim):
+    """More queries than keys under a causal mask: where the first key is seen, a
+    CTA has a tile of rows that see none (zeros) beside one of rows that do."""
+    lq = [4, 297, 5, 7, 55, 571, 3, 116, 9, 3, 34, 85, 21, 6, 17, 2, 635, 1500]
+    lk = [457, 667, 1338, 2193, 272, 42, 17, 114, 1123, 28, 1333, 24, 15, 48, 10, 20, 3, 700]
+    q, k, v = rand((sum(lq), heads, dim), 1, BF), rand((sum(lk), kv, dim), 2, BF), rand((sum(lk), kv, dim), 3, BF)
+    sq, sk = offsets(lq), offsets(lk)
+    ref = reference(q, k, v, spans(sq, sk), True, dim**-0.5)
+    for _ in range(5):
+        check(q, k, v, sq, sk, max(lk), ref=ref)
+
+
 def test_overlapping_query_ranges_read_nothing_outside_the_workspace():
     """Not allowed, and the rows' results mean nothing, but the lengths live on
     the device: a call whose ranges ask for more tiles than there are CTAs joins
