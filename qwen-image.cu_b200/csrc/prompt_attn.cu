@@ -17,7 +17,17 @@
 // warpgroup of softmax threads per tile (thread = row = TMEM lane).  Per 128-key
 // block and tile: S = Q K^T into TMEM (kind::f16, FP32), the softmax thread reads
 // its row, writes the weights as packed 16-bit over columns 0-63 of S, and
-// O += P V takes P from TMEM and V (token-major) from shared memory.
+// O += P V takes P from TMEM and V (token-major) from shared memory.  Two tiles'
+// S and O fill TMEM, so a tile's next S waits for its P V, and the other tile's
+// products run under its softmax.
+//
+// Measured (device time, calls in one graph): 8192 causal tokens, 28 heads on 4
+// of 128: 420-450 us, 1070-1150 TFLOP/s, tensor cores busy for 55% of the time;
+// 24 heads x 2 x 4352 keys: 435 us.  Bound by the chain S -> softmax -> P V of
+// each tile, not by the exponentials (polynomials for a part of them were
+// slower).  One token each against 16 caches of up to 4096: 23.4 us, one cache of
+// 30000: 23.3 us, of which reading K and V takes 9: the rest is set-up, the
+// first loads' latency and the joining launch.
 //
 // V guard.  A masked weight is 0, but 0 times a NaN or infinity of v is NaN: in
 // blocks with masked keys (the last ones) the guard clears the V rows that no
@@ -875,7 +885,9 @@ Plan plan_of(int heads, int kv_heads, int head_dim, int batch, int total_q, int 
   p.packs = G / p.P;
   const long long groups = heads / p.P;
   // One tile per CTA while those fit on the device at once (shorter calls) or
-  // sequences fill no second one; two over one K / V stream beyond that
+  // sequences fill no second one; two over one K / V stream beyond that.  One /
+  // two tiles: a pair of short prompts 7.2 / 9.0 us, one token for each of 16
+  // caches 24 / 27; packed prompts 107 / 78, 8192 causal tokens 714 / 453
   const long long ctas1 = (static_cast<long long>(total_q) / p.T + batch) * groups;
   p.nt = ctas1 <= num_sms || total_q < 2ll * p.T * batch ? 1 : 2;
   const long long units = static_cast<long long>(total_q) / (p.nt * p.T) + batch, ctas = units * groups;
