@@ -216,7 +216,8 @@ enum { QI_ACT_NONE = 0, QI_ACT_GELU = 1, QI_ACT_SILU = 2, QI_ACT_SWIGLU = 3 };
  * are in elements, positive and multiples of 8, pointers 16-byte aligned
  * (QI_ERR_ALIGN); rows and heads of out must not overlap one another.  total_q and
  * total_k are the rows of q / out and of k / v; ranges are clipped to them.
- * dtype is QI_DT_BF16 or QI_DT_F16 (all four tensors).  head_dim is a multiple
+ * dtype is QI_DT_BF16 or QI_DT_F16 (all four tensors); |scale| < 2e38
+ * (QI_ERR_ARG).  head_dim is a multiple
  * of 8, at most 128 (QI_ERR_UNSUPPORTED).  max_k >= the longest key range is a
  * hint that decides how keys are split over the device: a wrong one costs
  * time, not correctness.  workspace: at least

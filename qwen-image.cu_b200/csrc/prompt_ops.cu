@@ -77,7 +77,7 @@ extern "C" int qi_prompt_attention(const void* q, long long q_row, long long q_h
   int st = check_sizes(heads, kv_heads, head_dim, batch, total_q, total_k, max_k);
   if (st != QI_OK) return st;
   if (dtype != QI_DT_BF16 && dtype != QI_DT_F16) return QI_ERR_ARG;
-  if (!(scale > -3.0e38f && scale < 3.0e38f)) return QI_ERR_ARG;
+  if (!(scale > -2.0e38f && scale < 2.0e38f)) return QI_ERR_ARG;  // scale log2(e) is finite
   if (batch == 0 || total_q == 0) return QI_OK;
   if (!q || !out || !q_begin || !q_end || !k_begin || !k_end) return QI_ERR_ARG;
   if (total_k > 0 && (!k || !v)) return QI_ERR_ARG;

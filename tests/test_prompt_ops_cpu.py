@@ -115,3 +115,10 @@ def test_attention_refuses_overlaps_and_extents(kw, status):
                                 dict(N=(1 << 30) + 8, ldo=(1 << 30) + 8)])
 def test_linear_refuses_extents(kw):
     assert linear(**kw) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("scale", [2.9e38, -2.9e38, 2.5e38])
+def test_attention_refuses_scales_past_fp32_in_base_2(scale):
+    """scale * log2(e) would be infinite, and times a score of 0 not a number."""
+    assert attention(scale=scale) == ARG
+    assert attention(scale=scale / 2, total_q=0) == 0
