@@ -114,14 +114,24 @@ constexpr int BM = 256, BN_MAX = 256;
 constexpr int A_BLOCK = 128 * BK * 2;  // this CTA's 128 rows of x, one K block
 constexpr int MMA_WARP = 2, EPI_WARP0 = 3, EPI_WARPS = 8;  // warps 0 and 1 produce
 constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS);
-// Long sums (FP32 outputs, K > 4096).  The tensor cores round every addition to
-// an accumulator towards zero, so its error grows with K: measured 1.6e-5 of the
-// product at K = 14336.  There the epilogue warps take the accumulator over every
-// 2048 of K and add it, rounding to nearest, to a sum that also lives in TMEM
-// (error as at K = 2048: 2e-6).  Two accumulators and the sum are 3 x 160 of the
-// 512 columns, so these tiles are at most 160 wide (SwiGLU: 128).  16-bit outputs
-// do not see the error.
-constexpr int SUMS_MIN_K = 4096, SUMS_STEP = 2048 / BK;
+// Long sums.  The tensor cores truncate every addition to an accumulator, so its
+// error grows with K: 1e-9 K of the product in norm, 6.7e-9 K where all products
+// have one sign (BF16; measured: 2.1e-6 at K = 2048, 4.4e-6 at 4096, 1.6e-5 at
+// 14336; one sign 6.9e-3 at 2^20).  Where that would show, the epilogue warps take
+// the accumulator over every 2048 of K and add it, rounding to nearest, to a sum
+// that also lives in TMEM: the error stays that of K = 2048, and no warp waits for
+// more of K than that at once.  Two accumulators and the sum are 3 x 160 of the
+// 512 columns, so these tiles are at most 160 wide (SwiGLU: 128).
+// It shows in FP32 outputs from K = 2048 on, but they start at 4096, because up to
+// there it costs more than a factor of two in the error is worth: K 3584, 1024 /
+// 8192 x 3584 24.5 / 146 us without, 33.7 / 166 with parts, SwiGLU 1111 x 14336 171
+// and 225.  In 16-bit outputs it shows where it reaches a quarter of the half
+// step that they are rounded by, with one sign at K = 16384 (FP16) or 131072 (BF16).
+constexpr int SUMS_STEP = 2048 / BK;
+template <typename O>
+constexpr int sums_min_k() {
+  return std::is_same<O, float>::value ? 4096 : (std::is_same<O, __half>::value ? 16384 : 131072);
+}
 constexpr int SUMS_BN = 160, SUMS_BN_WIDE = 128;
 // staging sub-tile of one epilogue warp: 32 rows x 32 columns of the output
 template <typename O>
@@ -541,6 +551,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
 namespace rk {
 constexpr int WARPS = 8, THREADS = 32 * WARPS;
 constexpr int UNROLL = 4;  // 32-k blocks whose loads are in flight per warp
+// Steps of the K loop after which a warp adds its accumulators, rounding to
+// nearest, to its sums in shared memory: 2048 of its K, 16384 of the whole (see
+// Long sums above; one sign, K = 2^20: 8.6e-4 of the product without it).
+constexpr int SUMS_STEPS = 2048 / (32 * UNROLL);
 }  // namespace rk
 
 template <typename T>
@@ -623,6 +637,22 @@ __global__ void __launch_bounds__(rk::THREADS) linear16_rows_kernel(const __grid
 
   float acc[R][G][4] = {};
   const int kblocks = (args.K + 31) / 32;
+  // this thread's sums: its accumulators, added to what it had put there before
+  bool summed = false;
+  auto put = [&]() {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int j = 0; j < G; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float* p = red + (warp * 8 * G + 8 * j + 2 * t + (e & 1)) * STRIDE + 16 * r + g + 8 * (e >> 1);
+          *p = summed ? *p + acc[r][j][e] : acc[r][j][e];
+          acc[r][j][e] = 0.0f;
+        }
+    summed = true;
+  };
+  int steps = 0;
 #pragma unroll 1
   for (int kb = warp; kb < kblocks; kb += WARPS * UNROLL) {
     uint4 w[UNROLL][R][2];
@@ -648,14 +678,12 @@ __global__ void __launch_bounds__(rk::THREADS) linear16_rows_kernel(const __grid
         }
       }
     }
+    if (++steps == SUMS_STEPS) {
+      steps = 0;
+      put();
+    }
   }
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int j = 0; j < G; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        red[(warp * 8 * G + 8 * j + 2 * t + (e & 1)) * STRIDE + 16 * r + g + 8 * (e >> 1)] = acc[r][j][e];
+  put();
   __syncthreads();
   if (!in) return;
 #pragma unroll
@@ -805,8 +833,7 @@ int launch_typed(const Linear16Args& a, cudaStream_t stream) {
   d.N = a.N;
   d.K = a.K;
   d.act = a.act;
-  if constexpr (sizeof(O) == 4)
-    if (a.K > pk::SUMS_MIN_K) return launch_pair16<T, O, true>(a, d, stream, device_num_sms());
+  if (a.K > pk::sums_min_k<O>()) return launch_pair16<T, O, true>(a, d, stream, device_num_sms());
   return launch_pair16<T, O, false>(a, d, stream, device_num_sms());
 }
 

@@ -1,0 +1,69 @@
+"""Accuracy of qi_linear_16bit's FP32 sums against 64 bits, for long K and in
+norm: sharper than the element bounds of a K-long sum, which grow with K.
+
+The tensor cores truncate: every product and every running sum of a part of
+the kernel's 2048 values of K loses at most one step of 2^-23 of that sum; the
+parts' sums (K / 2048 at most, and 8 warps') are rounded to nearest, again at
+most 2^-23 each.
+"""
+import pytest
+import torch
+
+import qib200 as Q
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def rand(shape, seed, dtype=F32, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(HF, HF), (BF, BF), (HF, F32), (BF, F32)])
+@pytest.mark.parametrize("M", [1, 8, 16, 17, 300])
+@pytest.mark.parametrize("act", [Q.ACT_NONE, Q.ACT_SWIGLU])
+def test_long_sums_of_one_sign(dtype, out_dtype, M, act):
+    """A million products of one sign: a single truncated sum would lose 7e-3 of
+    them (measured), so would its 16-bit result.  Per element, with T the sum
+    and h the half step of out: e = (2048 + K / 2048 + 16) 2^-23 T; silu of these
+    sums (about 40) is the sum itself, plus 2^-19; SwiGLU multiplies two of them."""
+    K, N = (1 << 20) + 8, 32
+    wide = 2 if act == Q.ACT_SWIGLU else 1
+    x, w = rand((M, K), 1, dtype, 2.0**-7).abs(), rand((wide * N, K), 2, dtype, 2.0**-7).abs()
+    t = x.double() @ w.double().T
+    assert 30 < float(t.min()) and float(t.max()) < 60
+    e = (2048 + K / 2048 + 16) * 2**-23 * t
+    want = t
+    if act == Q.ACT_SWIGLU:
+        s, u = t[:, :N] * torch.sigmoid(t[:, :N]), t[:, N:]
+        es = e[:, :N] + 2**-19 * s
+        want, e = s * u, es * u + (s + es) * e[:, N:] + 2**-23 * s * u
+    tol = e + torch.finfo(out_dtype).eps / 2 * (want + e)
+    got = Q.linear_16bit(x, w, act=act, out_dtype=out_dtype)
+    torch.cuda.synchronize()
+    Q.prompt_ops_check()
+    assert float(((got.double() - want).abs() / tol).max()) <= 1
+
+
+@pytest.mark.parametrize("out_dtype,K", [(HF, 16392), (HF, 20480), (BF, 131080), (BF, 135168)])
+@pytest.mark.parametrize("M,N", [(130, 328), (2100, 1000)])
+def test_first_lengths_in_parts(out_dtype, K, M, N):
+    """The first K from which 16-bit outputs are made of parts, with everything in
+    the epilogue, in a CTA pair's first tile and in later ones."""
+    dtype = out_dtype
+    x, w = rand((M, K), 3, dtype), rand((N, K), 4, dtype, K**-0.5)
+    bias, gate, res = rand((N,), 5, dtype), rand((N,), 6), rand((M, N), 7, out_dtype)
+    t = x.double().abs() @ w.double().abs().T + bias.double().abs()
+    y = (x.double() @ w.double().T + bias.double()) * gate.double()
+    e = (2048 + K / 2048 + 17) * 2**-23 * t * gate.double().abs() + 2**-23 * y.abs()
+    want = y + res.double()
+    e = e + 2**-23 * want.abs()
+    tol = e + torch.finfo(out_dtype).eps / 2 * (want.abs() + e)
+    stream = res.clone()
+    got = Q.linear_16bit(x, w, bias=bias, gate=gate, residual=stream, out=stream)
+    torch.cuda.synchronize()
+    Q.prompt_ops_check()
+    assert got.data_ptr() == stream.data_ptr()
+    assert float(((got.double() - want).abs() / tol).max()) <= 1
