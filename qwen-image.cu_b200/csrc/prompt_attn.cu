@@ -1,9 +1,10 @@
 // prompt_attn.cu -- softmax attention over packed sequences with grouped heads,
 // on the 5th-generation tensor cores.
 //
-// For one query row with scores s_j = scale log2(e) q.k_j over the keys it sees:
-// running maximum m and sum l (FP32, base 2), weights 2^(s_j - m) rounded to the
-// 16-bit type, O = sum of weights times v in FP32, out = O / l.
+// For one query row with products r_j = q.k_j over the keys it sees and sc =
+// scale log2(e): running maximum m of the r_j and sum l (FP32), weights
+// 2^(sc (r_j - m)) rounded to the 16-bit type, O = sum of weights times v in FP32,
+// out = O / l.
 //
 // Work split.  The heads of a group read the same keys, so a 128-row query tile
 // holds T = 128 / P tokens of P heads of one group (P = the group's size up to
@@ -38,6 +39,7 @@
 #include "sm100.cuh"
 
 #include <limits.h>
+#include <math.h>
 
 #include <type_traits>
 
@@ -72,9 +74,10 @@ struct alignas(64) PromptAttnDev {
   int items;         // work items per head pack at most: (unit of NT tiles, split of its keys) (gridDim.x)
   int splits;        // splits of a sequence's keys at most
   float sc;          // |scale| log2(e)
+  float step;        // 8 / sc: what a row's maximum grows by before it moves
   uint32_t negate;   // scale < 0: instruction descriptor bit 13 (negate A) for Q K^T
   float* part;       // splits > 1: [splits][total_q * heads][DH] normalised partial outputs
-  float2* ml;        // splits > 1: [splits][total_q * heads] (m, l)
+  float2* ml;        // splits > 1: [splits][total_q * heads] (m, l), m before scaling
   int* used;         // splits > 1: [total_q * heads] splits that hold the row's keys
 };
 
@@ -555,6 +558,8 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
     // FP16 weights are kept in 2^7 .. 2^15 for the largest so that small ones
     // stay clear of the subnormals; the factor is in l too
     constexpr float LIFT = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+    // scores in base 2 up to which sc m may be rounded (off by 2^-16 at most)
+    constexpr float FAR = 256.0f;
     const uint64_t sc2 = f2pack(args.sc, args.sc);
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
@@ -594,11 +599,11 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
         for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(r[BKV - 4 + e]));
         const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
         // Lazy rescale: the maximum used moves only when the row's grows by more
-        // than 8 (weights stay <= 2^8); O and l move with it
-        const float m_new = fmaxf(m, top == -INFINITY ? -INFINITY : top * args.sc);
-        const bool grow = m_new > m + 8.0f;
+        // than 8 in base 2 (weights stay <= 2^8); O and l move with it
+        const float m_new = fmaxf(m, top);
+        const bool grow = m_new - m > args.step;
         if (grow) {
-          alpha = ex2(m - m_new);
+          alpha = ex2((m - m_new) * args.sc);
           m = m_new;
         }
         if (i > 0 && __any_sync(0xffffffffu, grow)) {
@@ -613,27 +618,41 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
             tmem_st32(o_tm + c, o);
           }
         }
-        const float base = m == -INFINITY ? 0.0f : LIFT - m;  // nothing seen yet: every weight is 0
-        const uint64_t base2 = f2pack(base, base);
+        // Exponents sc (r - m): exact differences near the maximum, whatever its
+        // size.  Or in one step, sc r - sc m, where rounding sc m is no error worth
+        // minding.  With two tiles the first form is the faster one (8192 causal
+        // tokens 432 against 449 us), with one the second (16 single tokens 25.6
+        // against 24.2).  Nothing seen yet: every weight is 0
+        const float base = m == -INFINITY ? 0.0f : fmaf(-m, args.sc, LIFT);
+        auto weights = [&](auto exact_tag) {
+          constexpr bool EXACT = decltype(exact_tag)::value;
+          const float off = !EXACT ? base : (m == -INFINITY ? 0.0f : -m);
+          const uint64_t off2 = f2pack(off, off), lift2 = f2pack(LIFT, LIFT);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t pk[32];
+          for (int h = 0; h < 2; ++h) {
+            uint32_t pk[32];
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const int k = 64 * h + 2 * c;
-            float p0, p1;
-            f2unpack(f2fma(f2pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), sc2, base2), p0, p1);
-            p0 = ex2(p0);
-            p1 = ex2(p1);
-            sum2[c & 3] = f2add(sum2[c & 3], f2pack(p0, p1));
-            pk[c] = pack16<T>(p0, p1);
+            for (int c = 0; c < 32; ++c) {
+              const int k = 64 * h + 2 * c;
+              const uint64_t r2 = f2pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1]));
+              float p0, p1;
+              f2unpack(EXACT ? f2fma(f2add(r2, off2), sc2, lift2) : f2fma(r2, sc2, off2), p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+              sum2[c & 3] = f2add(sum2[c & 3], f2pack(p0, p1));
+              pk[c] = pack16<T>(p0, p1);
+            }
+            tmem_st32(s_tm + 32 * h, pk);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_half[2 * t + h]);
           }
-          tmem_st32(s_tm + 32 * h, pk);
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_half[2 * t + h]);
-        }
+        };
+        if (NT == 2 || __builtin_expect(__any_sync(0xffffffffu, valid && fabsf(base) > FAR), 0))
+          weights(std::true_type{});
+        else
+          weights(std::false_type{});
       };
       if (__any_sync(0xffffffffu, seen < BKV - 1))
         block(std::true_type{});
@@ -762,7 +781,7 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
   }
 }
 
-// Joins the splits of a row: out = sum_s w_s O_s / sum_s w_s, w_s = l_s 2^(m_s - max m).
+// Joins the splits of a row: out = sum_s w_s O_s / sum_s w_s, w_s = l_s 2^(sc (m_s - max m)).
 // A CTA per token and 8 / per heads; `per` warps per head take its splits in
 // turn, four dimensions per thread, and add up in warp order.  Rows whose tile
 // had one split are final already.
@@ -776,6 +795,7 @@ struct JoinDev {
   const int* used;
   int batch, total_q, heads, head_dim;
   int warps, splits;  // warps per head; splits the workspace holds
+  float sc;
 };
 template <typename T, int DH>
 __global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_constant__ JoinDev args) {
@@ -822,11 +842,11 @@ __global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_cons
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
     t = fmaxf(t, top);
-    const float keep = top == -INFINITY ? 0.0f : ex2(top - t);
+    const float keep = top == -INFINITY ? 0.0f : ex2((top - t) * args.sc);
     top = t;
     total *= keep;
     o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
-    const float w_lane = ml.y == 0.0f ? 0.0f : ml.y * ex2(ml.x - top);
+    const float w_lane = ml.y == 0.0f ? 0.0f : ml.y * ex2((ml.x - top) * args.sc);
     const int ahead = per > 1 && i0 == 0 ? min(mine, AHEAD) : 0;
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
@@ -857,7 +877,7 @@ __global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_cons
     for (int i = 0; i < per; ++i) {
       const float2 tw = part_w[warp + i];
       if (tw.x == -INFINITY && tw.y == 0.0f) continue;
-      const float k = ex2(tw.x - top);
+      const float k = ex2((tw.x - top) * args.sc);
       const float4 v = part_o[warp + i][lane];
       total += k * tw.y;
       o = make_float4(o.x + k * v.x, o.y + k * v.y, o.z + k * v.z, o.w + k * v.w);
@@ -949,7 +969,7 @@ int launch_tiles(const PromptAttnDev& d, cudaStream_t stream) {
   while (warps > 1 && rows * warps > 8192) warps /= 2;
   const int per_cta = 8 / warps;
   const JoinDev j{a.out, a.o_row, a.o_head, a.q_begin, a.q_end, d.part, d.ml, d.used, a.batch, a.total_q, a.heads, a.head_dim,
-                  warps, d.splits};
+                  warps, d.splits, d.sc};
   return launch_dependent(prompt_attn_join_kernel<T, DH>, dim3(a.total_q, (a.heads + per_cta - 1) / per_cta), 256, 0, j, stream);
 }
 
@@ -983,6 +1003,7 @@ int prompt_attention_launch(const PromptAttnArgs& a, cudaStream_t stream) {
   // scale 0: the smallest normal number does the same to finite scores (every
   // weight 1) and leaves masked ones at -inf, where 0 would make them NaN
   if (d.sc < 1.17549435e-38f) d.sc = 1.17549435e-38f;
+  d.step = fminf(8.0f / d.sc, 3.4028235e38f);
   d.negate = a.scale < 0.0f ? 1u << 13 : 0u;
   if (p.splits > 1) {
     const long long rows = static_cast<long long>(a.total_q) * a.heads;
