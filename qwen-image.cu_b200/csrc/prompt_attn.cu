@@ -86,6 +86,23 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Products with sc, which may be subnormal: without the flushing to zero that
+// this build's own multiplications have.
+__device__ __forceinline__ float mul_sub(float a, float b) {
+  float y;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float fma_sub(float a, float b, float c) {
+  float y;
+  asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+__device__ __forceinline__ uint64_t f2fma_sub(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+  return y;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -603,7 +620,7 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
         const float m_new = fmaxf(m, top);
         const bool grow = m_new - m > args.step;
         if (grow) {
-          alpha = ex2((m - m_new) * args.sc);
+          alpha = ex2(mul_sub(m - m_new, args.sc));
           m = m_new;
         }
         if (i > 0 && __any_sync(0xffffffffu, grow)) {
@@ -623,7 +640,7 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
         // minding.  With two tiles the first form is the faster one (8192 causal
         // tokens 432 against 449 us), with one the second (16 single tokens 25.6
         // against 24.2).  Nothing seen yet: every weight is 0
-        const float base = m == -INFINITY ? 0.0f : fmaf(-m, args.sc, LIFT);
+        const float base = m == -INFINITY ? 0.0f : fma_sub(-m, args.sc, LIFT);
         auto weights = [&](auto exact_tag) {
           constexpr bool EXACT = decltype(exact_tag)::value;
           const float off = !EXACT ? base : (m == -INFINITY ? 0.0f : -m);
@@ -636,7 +653,7 @@ __global__ void __launch_bounds__(Cfg<DH, NT>::THREADS, Cfg<DH, NT>::MIN_CTAS)
               const int k = 64 * h + 2 * c;
               const uint64_t r2 = f2pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1]));
               float p0, p1;
-              f2unpack(EXACT ? f2fma(f2add(r2, off2), sc2, lift2) : f2fma(r2, sc2, off2), p0, p1);
+              f2unpack(EXACT ? f2fma_sub(f2add(r2, off2), sc2, lift2) : f2fma_sub(r2, sc2, off2), p0, p1);
               p0 = ex2(p0);
               p1 = ex2(p1);
               sum2[c & 3] = f2add(sum2[c & 3], f2pack(p0, p1));
@@ -842,11 +859,11 @@ __global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_cons
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
     t = fmaxf(t, top);
-    const float keep = top == -INFINITY ? 0.0f : ex2((top - t) * args.sc);
+    const float keep = top == -INFINITY ? 0.0f : ex2(mul_sub(top - t, args.sc));
     top = t;
     total *= keep;
     o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
-    const float w_lane = ml.y == 0.0f ? 0.0f : ml.y * ex2((ml.x - top) * args.sc);
+    const float w_lane = ml.y == 0.0f ? 0.0f : ml.y * ex2(mul_sub(ml.x - top, args.sc));
     const int ahead = per > 1 && i0 == 0 ? min(mine, AHEAD) : 0;
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
@@ -877,7 +894,7 @@ __global__ void __launch_bounds__(256) prompt_attn_join_kernel(const __grid_cons
     for (int i = 0; i < per; ++i) {
       const float2 tw = part_w[warp + i];
       if (tw.x == -INFINITY && tw.y == 0.0f) continue;
-      const float k = ex2((tw.x - top) * args.sc);
+      const float k = ex2(mul_sub(tw.x - top, args.sc));
       const float4 v = part_o[warp + i][lane];
       total += k * tw.y;
       o = make_float4(o.x + k * v.x, o.y + k * v.y, o.z + k * v.z, o.w + k * v.w);
@@ -1000,9 +1017,11 @@ int prompt_attention_launch(const PromptAttnArgs& a, cudaStream_t stream) {
   d.items = static_cast<int>(p.items);
   d.splits = p.splits;
   d.sc = (a.scale < 0.0f ? -a.scale : a.scale) * 1.4426950408889634f;
-  // scale 0: the smallest normal number does the same to finite scores (every
-  // weight 1) and leaves masked ones at -inf, where 0 would make them NaN
-  if (d.sc < 1.17549435e-38f) d.sc = 1.17549435e-38f;
+  // scale 0: the smallest subnormal number.  No finite score makes an exponent
+  // past 2^-20 with it (weights 1), and masked scores stay at -inf, where 0 would
+  // make them NaN
+  constexpr float TINY = 1.40129846e-45f;
+  if (d.sc < TINY) d.sc = TINY;
   d.step = fminf(8.0f / d.sc, 3.4028235e38f);
   d.negate = a.scale < 0.0f ? 1u << 13 : 0u;
   if (p.splits > 1) {

@@ -97,3 +97,15 @@ def test_maximum_that_comes_late(dtype):
     ramp = torch.arange(5000, device="cuda") // 16 * 4.0 - 500
     k[:, :, 0] = (ramp.clamp(max=200)[:, None]).to(dtype)
     check(q, k, v, lq, lk, 0.05)
+
+
+@pytest.mark.parametrize("dtype,big", [(BF, 2.0**62), (HF, 2.0**14)])
+@pytest.mark.parametrize("lq,lk", CALLS)
+@pytest.mark.parametrize("scale", [0.0, 2.0**-126, -(2.0**-127), 2.0**-128, 2.0**-140, 2.0**-149])
+def test_smallest_scales(dtype, big, lq, lk, scale):
+    """Scales down to the smallest subnormal number: with scores up to 3 x 2^124
+    (BF16) they still decide, and scale 0 weighs all keys alike."""
+    q, k, v = whole((sum(lq), 14, 64), 10, dtype, 3), whole((sum(lk), 2, 64), 11, dtype, 3), normal((sum(lk), 2, 64), 12, dtype)
+    q[:, :, 1:], k[:, :, 1:] = 0, 0
+    q[:, :, 0], k[:, :, 0] = big, k[:, :, 0] * big
+    check(q, k, v, lq, lk, scale)
