@@ -974,6 +974,21 @@ int launch_tiles(const PromptAttnDev& d, cudaStream_t stream) {
   static_assert(C::SMEM <= 227 * 1024, "shared memory");
   static unsigned long long attr_done = 0;
   const auto fn = prompt_attn_kernel<T, DH, NT>;
+  if (C::LAUNCH_REGS < 256) {
+    // The register split counts on LAUNCH_REGS per thread at launch: with fewer,
+    // the softmax warps would wait for theirs without end.  A build that gave the
+    // kernel another number is refused
+    static int checked = 0;
+    if (!__atomic_load_n(&checked, __ATOMIC_ACQUIRE)) {
+      cudaFuncAttributes fa;
+      if (cudaFuncGetAttributes(&fa, reinterpret_cast<const void*>(fn)) != cudaSuccess) {
+        cudaGetLastError();
+        return QI_ERR_CUDA;
+      }
+      if (fa.numRegs != C::LAUNCH_REGS) return QI_ERR_UNSUPPORTED;
+      __atomic_store_n(&checked, 1, __ATOMIC_RELEASE);
+    }
+  }
   if (smem_optin(reinterpret_cast<const void*>(fn), C::SMEM, &attr_done) != QI_OK) return QI_ERR_CUDA;
   const dim3 grid(d.items, d.a.heads / d.P);
   const int st = launch_dependent(fn, grid, C::THREADS, C::SMEM, d, stream);
