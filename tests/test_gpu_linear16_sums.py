@@ -67,3 +67,42 @@ def test_first_lengths_in_parts(out_dtype, K, M, N):
     Q.prompt_ops_check()
     assert got.data_ptr() == stream.data_ptr()
     assert float(((got.double() - want).abs() / tol).max()) <= 1
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("M", [1, 3, 8, 9, 16, 17, 130, 600])
+@pytest.mark.parametrize("K", [64, 1000, 2048, 3584, 4096, 4104, 18944])
+def test_fp32_results_in_norm(dtype, M, K):
+    """FP32 outputs of every kernel and epilogue in norm, with random signs.  Of n
+    additions to one sum, which grows as the square root of their number, each
+    loses at most 2^-23 of it: 2/3 n 2^-23 of the result.  n = K / 16, parts of
+    2048 from K > 4096 on; with up to 16 rows eight warps share K.  A sum of few
+    terms, of parts or of warps adds 2^-22.  The loss goes with the sums' size s,
+    not with the result's: under a slope of 1.13 (silu, GELU) or times the other
+    factor (SwiGLU) it is s times theirs; their own arithmetic adds 2^-18."""
+    N = 328
+    x, w, w2 = rand((M, K), 11, dtype), rand((N, K), 12, dtype, K**-0.5), rand((N, K), 13, dtype, K**-0.5)
+    bias, gate, res = rand((N,), 14, dtype), rand((N,), 15), rand((M, N), 16)
+    tiles = (2048 if K > 4096 else K) / 16
+    n, n_wide = (K / 128 if M <= most else tiles for most in (16, 8))  # SwiGLU: up to 8 rows
+    b, b_wide = (2 / 3 * m * 2**-23 + 2**-22 for m in (n, n_wide))
+    a, u = x.double() @ w.double().T, x.double() @ w2.double().T
+
+    def close(got, want, bound):
+        torch.cuda.synchronize()
+        Q.prompt_ops_check()
+        assert got.dtype == F32
+        assert float((got.double() - want).norm()) <= bound
+
+    close(Q.linear_16bit(x, w, out_dtype=F32), a, b * a.norm())
+    y = (a + bias.double()) * gate.double()
+    close(Q.linear_16bit(x, w, bias=bias, gate=gate, residual=res, out_dtype=F32), y + res.double(),
+          b * (a * gate.double()).norm() + 2**-22 * (y.norm() + res.double().norm()))
+    size = a.square().mean().sqrt() * a.numel() ** 0.5
+    silu = a * torch.sigmoid(a)
+    close(Q.linear_16bit(x, w, act=Q.ACT_SILU, out_dtype=F32), silu, 1.13 * b * size + 2**-18 * silu.norm())
+    gelu = a * torch.sigmoid(2 * (2 / torch.pi) ** 0.5 * (a + 0.044715 * a**3))
+    close(Q.linear_16bit(x, w, act=Q.ACT_GELU, out_dtype=F32), gelu, 1.13 * b * size + 2**-18 * gelu.norm())
+    s = a.square().mean().sqrt()
+    close(Q.linear_16bit(x, torch.cat([w, w2]), act=Q.ACT_SWIGLU, out_dtype=F32), silu * u,
+          b_wide * s * (1.13 * u.norm() + silu.norm()) + 2**-18 * (silu * u).norm())
