@@ -28,9 +28,7 @@ struct alignas(64) L16Dev {  // pair kernel
   CUtensorMap tmX, tmW, tmO, tmR;  // x, w, output, residual
   const void* bias;
   const float* gate;
-  const void* residual;
-  void* out;
-  long long ldr, ldo;
+  const void* residual;  // NULL: none (read through tmR)
   int M, N, K, act;
   int stages, atoms;  // TMA pipeline depth, K blocks per stage
   int bn, tiles_m, tiles_n;
@@ -804,10 +802,8 @@ template <typename T, typename O, int G, int R, bool WIDE>
 int launch_rows(const Linear16Args& a, cudaStream_t stream) {
   constexpr int COLS = WIDE ? 16 : 16 * R;
   constexpr int smem = rk::WARPS * 8 * G * (16 * R + 4) * 4;
-  static unsigned long long attr_done = 0;
-  const auto fn = linear16_rows_kernel<T, O, G, R, WIDE>;
-  if (smem > 48 * 1024 && smem_optin(reinterpret_cast<const void*>(fn), smem, &attr_done) != QI_OK) return QI_ERR_CUDA;
-  return launch16(fn, static_cast<unsigned>((a.N + COLS - 1) / COLS), rk::THREADS, smem, a, stream);
+  static_assert(smem <= 48 * 1024, "shared memory that needs no opt-in");
+  return launch16(linear16_rows_kernel<T, O, G, R, WIDE>, static_cast<unsigned>((a.N + COLS - 1) / COLS), rk::THREADS, smem, a, stream);
 }
 
 template <typename T, typename O>
@@ -826,9 +822,6 @@ int launch_typed(const Linear16Args& a, cudaStream_t stream) {
   d.bias = a.bias;
   d.gate = a.gate;
   d.residual = a.residual;
-  d.out = a.out;
-  d.ldr = a.ldr;
-  d.ldo = a.ldo;
   d.M = a.M;
   d.N = a.N;
   d.K = a.K;
