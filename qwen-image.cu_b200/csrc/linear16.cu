@@ -110,27 +110,34 @@ __device__ __forceinline__ void add_bias32(float (&v)[32], const T* p, int n_val
 namespace pk {
 constexpr int BM = 256, BN_MAX = 256;
 constexpr int A_BLOCK = 128 * BK * 2;  // this CTA's 128 rows of x, one K block
-constexpr int MMA_WARP = 2, EPI_WARP0 = 3, EPI_WARPS = 8;  // warps 0 and 1 produce
+constexpr int MMA_WARP = 2, EPI_WARP0 = 4, EPI_WARPS = 8;  // warps 0 and 1 produce, 3 has no part
 constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS);
-// Long sums.  The tensor cores truncate every addition to an accumulator, so its
-// error grows with K: 1e-9 K of the product in norm, 6.7e-9 K where all products
-// have one sign (BF16; measured: 2.1e-6 at K = 2048, 4.4e-6 at 4096, 1.6e-5 at
-// 14336; one sign 6.9e-3 at 2^20).  Where that would show, the epilogue warps take
-// the accumulator over every 2048 of K and add it, rounding to nearest, to a sum
-// that also lives in TMEM: the error stays that of K = 2048, and no warp waits for
-// more of K than that at once.  Two accumulators and the sum are 3 x 160 of the
-// 512 columns, so these tiles are at most 160 wide (SwiGLU: 128).
-// It shows in FP32 outputs from K = 2048 on, but they start at 4096, because up to
-// there it costs more than a factor of two in the error is worth: K 3584, 1024 /
-// 8192 x 3584 24.5 / 146 us without, 33.7 / 166 with parts, SwiGLU 1111 x 14336 171
-// and 225.  In 16-bit outputs it shows where it reaches a quarter of the half
-// step that they are rounded by, with one sign at K = 16384 (FP16) or 131072 (BF16).
-constexpr int SUMS_STEP = 2048 / BK;
-template <typename O>
-constexpr int sums_min_k() {
-  return std::is_same<O, float>::value ? 4096 : (std::is_same<O, __half>::value ? 16384 : 131072);
+// sums in parts: registers per thread at launch, then of the first warpgroup and
+// of the epilogue's two
+constexpr int LAUNCH_REGS = 168, PRODUCER_REGS = 88, EPI_REGS = 208;
+static_assert(32 * (EPI_WARP0 * PRODUCER_REGS + EPI_WARPS * EPI_REGS) <= THREADS * LAUNCH_REGS, "register split exceeds the launch");
+// Sums in parts.  The tensor cores truncate every addition to an accumulator, so
+// its error grows with K: 9e-10 K (BF16) or 1.3e-9 K (FP16) of the product in norm,
+// with one sign 1.6e-9 or 5e-9 K at small K, 6.7e-9 K (FP16) at large.  Where that
+// would show, the epilogue warps take the accumulator over every 768 (BF16) or 512
+// (FP16) of K and add it, rounding to nearest, to sums in their registers (128 per
+// thread for a 256 x 256 tile); the last part's total goes back to TMEM, where the
+// epilogue finds it.  SwiGLU, whose two factors lose in the same direction, takes
+// half of that.  Norm error 8e-7 at most for every K, and no warp waits for more of
+// K than a part at once.  A part costs 0.24 us, the first MMA on the other
+// accumulator (M 8192, N = K = 3584: 148 us as one sum, error 3.9e-6; 156 with
+// parts of 768, 163 of 512; SwiGLU, M 1111, N 14336: 172 as one sum, 201).
+// It shows in FP32 outputs from one part on; in 16-bit outputs where it reaches a
+// quarter of the half step that they are rounded by, with one sign at K = 16384
+// (FP16) or 131072 (BF16).
+template <typename T>
+constexpr int sums_step(bool wide) {  // K blocks, even
+  return (std::is_same<T, __half>::value ? 512 : 768) / (wide ? 2 : 1) / BK;
 }
-constexpr int SUMS_BN = 160, SUMS_BN_WIDE = 128;
+template <typename T, typename O>
+constexpr int sums_min_k(bool wide) {
+  return std::is_same<O, float>::value ? BK * sums_step<T>(wide) : (std::is_same<O, __half>::value ? 16384 : 131072);
+}
 // staging sub-tile of one epilogue warp: 32 rows x 32 columns of the output
 template <typename O>
 constexpr int sub_bytes() { return 32 * 32 * static_cast<int>(sizeof(O)); }
@@ -155,7 +162,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
     linear16_pair_kernel(const __grid_constant__ L16Dev args) {
   using namespace pk;
   constexpr int SUB = sub_bytes<O>();
-  constexpr int ACC = SUMS ? SUMS_BN : BN_MAX;  // TMEM columns of an accumulator; SUMS: the sum at 2 ACC
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int stages = args.stages, atoms = args.atoms;
@@ -181,7 +187,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
   const bool wide = args.act == QI_ACT_SWIGLU;
   const int bn_out = wide ? bn / 2 : bn;
   const int kblocks = (args.K + BK - 1) / BK;
-  const int kstep = SUMS ? SUMS_STEP : kblocks;  // K blocks per accumulator
+  const int kstep = SUMS ? sums_step<T>(wide) : kblocks;  // K blocks per accumulator
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
@@ -213,112 +219,116 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
   grid_dependency_wait();
   launch_dependents();
 
-  if (warp < MMA_WARP) {
-    // ------------------------------------------------------------ producers (both CTAs)
-    // Warp 0 brings x, warp 1 brings w: waiting for a stage and issuing both
-    // copies takes one thread ~430 clocks, more than a narrow tile's MMAs.
-    if (lane == 0) {
-      const uint32_t full0 = mapa_shared(&full[0], 0);  // the even CTA's stage barriers
-      const uint32_t stage_tx = 2 * (a_bytes + b_bytes);  // both CTAs' bytes
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int t = cluster; t < total && ok; t += nclusters) {
-        int m0, nt;
-        pair_tile(args, t, m0, nt);
-        // SwiGLU: the even CTA brings the tile's gate rows of w, the odd CTA
-        // its up rows, so accumulator columns [0, bn/2) are the gate products
-        const int wrow = wide ? nt * bn_out + static_cast<int>(cr) * args.N : nt * bn + (bn / 2) * static_cast<int>(cr);
-        const int row = warp == 0 ? m0 + 128 * static_cast<int>(cr) : wrow;
-        const CUtensorMap* tm = warp == 0 ? &args.tmX : &args.tmW;
-        uint8_t* dst = warp == 0 ? sA : sB;
-        const int block = warp == 0 ? A_BLOCK : b_block;
-        for (int kb = 0; kb < kblocks; kb += atoms) {
-          if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag)) {
-            ok = false;
-            break;
-          }
-          if (leader && warp == 0) mbar_expect_tx(&full[stage], stage_tx);
-          uint8_t* to = dst + stage * atoms * block;
-          tma_load_2d_pair(to, tm, kb * BK, row, full0 + stage * 8);
-          if (atoms == 2) tma_load_2d_pair(to + block, tm, (kb + 1) * BK, row, full0 + stage * 8);  // past K: zeros
-          if (++stage == stages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-      }
-      if (!ok) {
-        *abort_flag = 1;
-        atomicCAS(&g_linear16_err, 0, kErrTimeoutProducer);
-        // copies already issued complete on the even CTA's barrier: give them
-        // time to land before this CTA leaves
-        const uint64_t t0 = global_timer_ns();
-        while (global_timer_ns() - t0 < 200000ull) {
-        }
-      }
-    }
-  } else if (warp == MMA_WARP) {
-    // ------------------------------------------------------------ MMA issuer (even CTA)
-    if (leader) {
-      auto wait_all = [&](uint64_t* bar, uint32_t parity) {
-        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
-      };
-      int stage = 0, local = 0;
-      uint32_t phase = 0;
-      bool ok = true, ready = mbar_test_wait(&full[0], 0);
-      const uint32_t idesc = idesc16<T>(BM, 0) | (static_cast<uint32_t>(bn >> 3) << 17);
-      const uint64_t ad0 = umma_desc_sw128(smem_u32(sA), 16, 1024), bd0 = umma_desc_sw128(smem_u32(sB), 16, 1024);
-      for (int t = cluster; t < total && ok; t += nclusters) {
-        for (int k0 = 0; k0 < kblocks && ok; k0 += kstep, ++local) {
-          const int buf = local & 1, k1 = min(kblocks, k0 + kstep);
-          if (!wait_all(&tempty[buf], ((local >> 1) & 1) ^ 1u)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t d_tmem = tmem_base + buf * ACC;
-          for (int kb = k0; kb < k1; kb += atoms) {
-            if (!__all_sync(0xffffffffu, ready) && !wait_all(&full[stage], phase)) {
+  if (warp < EPI_WARP0) {
+    if constexpr (SUMS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGS));
+    if (warp < MMA_WARP) {
+      // ------------------------------------------------------------ producers (both CTAs)
+      // Warp 0 brings x, warp 1 brings w: waiting for a stage and issuing both
+      // copies takes one thread ~430 clocks, more than a narrow tile's MMAs.
+      if (lane == 0) {
+        const uint32_t full0 = mapa_shared(&full[0], 0);  // the even CTA's stage barriers
+        const uint32_t stage_tx = 2 * (a_bytes + b_bytes);  // both CTAs' bytes
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int t = cluster; t < total && ok; t += nclusters) {
+          int m0, nt;
+          pair_tile(args, t, m0, nt);
+          // SwiGLU: the even CTA brings the tile's gate rows of w, the odd CTA
+          // its up rows, so accumulator columns [0, bn/2) are the gate products
+          const int wrow = wide ? nt * bn_out + static_cast<int>(cr) * args.N : nt * bn + (bn / 2) * static_cast<int>(cr);
+          const int row = warp == 0 ? m0 + 128 * static_cast<int>(cr) : wrow;
+          const CUtensorMap* tm = warp == 0 ? &args.tmX : &args.tmW;
+          uint8_t* dst = warp == 0 ? sA : sB;
+          const int block = warp == 0 ? A_BLOCK : b_block;
+          for (int kb = 0; kb < kblocks; kb += atoms) {
+            if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag)) {
               ok = false;
               break;
             }
-            tc_fence_after();
-            const int cur = stage;
+            if (leader && warp == 0) mbar_expect_tx(&full[stage], stage_tx);
+            uint8_t* to = dst + stage * atoms * block;
+            tma_load_2d_pair(to, tm, kb * BK, row, full0 + stage * 8);
+            if (atoms == 2) tma_load_2d_pair(to + block, tm, (kb + 1) * BK, row, full0 + stage * 8);  // past K: zeros
             if (++stage == stages) {
               stage = 0;
               phase ^= 1u;
             }
-            ready = mbar_test_wait(&full[stage], phase);
-            uint64_t ad = ad0 + static_cast<uint64_t>((cur * a_bytes) >> 4);
-            uint64_t bd = bd0 + static_cast<uint64_t>((cur * b_bytes) >> 4);
-#pragma unroll
-            for (int k = 0; k < BK / 16; ++k)
-              mma_f16_ss_pair_elect(d_tmem, ad + 2 * k, bd + 2 * k, idesc, kb > k0 || k > 0 ? 1u : 0u);
-            if (atoms == 2) {
-              ad += A_BLOCK >> 4;
-              bd += static_cast<uint64_t>(b_block >> 4);
-#pragma unroll
-              for (int k = 0; k < BK / 16; ++k) mma_f16_ss_pair_elect(d_tmem, ad + 2 * k, bd + 2 * k, idesc, 1u);
-            }
-            mma_commit_pair_elect(&empty[cur], 0x3);
           }
-          if (!ok) break;
-          mma_commit_pair_elect(&tfull[buf], 0x3);
+        }
+        if (!ok) {
+          *abort_flag = 1;
+          atomicCAS(&g_linear16_err, 0, kErrTimeoutProducer);
+          // copies already issued complete on the even CTA's barrier: give them
+          // time to land before this CTA leaves
+          const uint64_t t0 = global_timer_ns();
+          while (global_timer_ns() - t0 < 200000ull) {
+          }
         }
       }
-      if (!ok && lane == 0) {
-        *abort_flag = 1;
-        atomicCAS(&g_linear16_err, 0, kErrTimeoutMma);
-      }
-      __syncwarp();
-      // every MMA issued above (it writes both CTAs' TMEM) completes before teardown
-      mma_commit_pair_elect(drain, 0x1);
-      const uint64_t t0 = global_timer_ns();
-      while (!mbar_try_wait(drain, 0) && global_timer_ns() - t0 < kWaitLimitNs / 4) {
+    } else if (warp == MMA_WARP) {
+      // ------------------------------------------------------------ MMA issuer (even CTA)
+      if (leader) {
+        auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+          return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+        };
+        int stage = 0, local = 0;
+        uint32_t phase = 0;
+        bool ok = true, ready = mbar_test_wait(&full[0], 0);
+        const uint32_t idesc = idesc16<T>(BM, 0) | (static_cast<uint32_t>(bn >> 3) << 17);
+        const uint64_t ad0 = umma_desc_sw128(smem_u32(sA), 16, 1024), bd0 = umma_desc_sw128(smem_u32(sB), 16, 1024);
+        for (int t = cluster; t < total && ok; t += nclusters) {
+          for (int k0 = 0; k0 < kblocks && ok; k0 += kstep, ++local) {
+            const int buf = local & 1, k1 = min(kblocks, k0 + kstep);
+            if (!wait_all(&tempty[buf], ((local >> 1) & 1) ^ 1u)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t d_tmem = tmem_base + buf * BN_MAX;
+            for (int kb = k0; kb < k1; kb += atoms) {
+              if (!__all_sync(0xffffffffu, ready) && !wait_all(&full[stage], phase)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const int cur = stage;
+              if (++stage == stages) {
+                stage = 0;
+                phase ^= 1u;
+              }
+              ready = mbar_test_wait(&full[stage], phase);
+              uint64_t ad = ad0 + static_cast<uint64_t>((cur * a_bytes) >> 4);
+              uint64_t bd = bd0 + static_cast<uint64_t>((cur * b_bytes) >> 4);
+#pragma unroll
+              for (int k = 0; k < BK / 16; ++k)
+                mma_f16_ss_pair_elect(d_tmem, ad + 2 * k, bd + 2 * k, idesc, kb > k0 || k > 0 ? 1u : 0u);
+              if (atoms == 2) {
+                ad += A_BLOCK >> 4;
+                bd += static_cast<uint64_t>(b_block >> 4);
+#pragma unroll
+                for (int k = 0; k < BK / 16; ++k) mma_f16_ss_pair_elect(d_tmem, ad + 2 * k, bd + 2 * k, idesc, 1u);
+              }
+              mma_commit_pair_elect(&empty[cur], 0x3);
+            }
+            if (!ok) break;
+            mma_commit_pair_elect(&tfull[buf], 0x3);
+          }
+        }
+        if (!ok && lane == 0) {
+          *abort_flag = 1;
+          atomicCAS(&g_linear16_err, 0, kErrTimeoutMma);
+        }
+        __syncwarp();
+        // every MMA issued above (it writes both CTAs' TMEM) completes before teardown
+        mma_commit_pair_elect(drain, 0x1);
+        const uint64_t t0 = global_timer_ns();
+        while (!mbar_try_wait(drain, 0) && global_timer_ns() - t0 < kWaitLimitNs / 4) {
+        }
       }
     }
-  } else if (warp >= EPI_WARP0) {
+  } else {
+    if constexpr (SUMS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(EPI_REGS));
     // ------------------------------------------------------------ epilogue (both CTAs)
     // A warp owns 32 rows (its TMEM lane quarter, thread = row) and every
     // second 32-column chunk of the tile: TMEM -> registers -> bias,
@@ -347,59 +357,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
         tma_load_2d(ebuf + b * SUB, &args.tmR, n0 + 32 * half, r0, &xb[b]);
         xpending |= 1u << b;
       }
-      const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16), sum_tm = lanes + 2 * ACC;
+      const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
       bool w = true;
-      if constexpr (SUMS) {  // the accumulators before the tile's last one
-        for (int k0 = kstep; k0 < kblocks && ok; k0 += kstep, ++local) {
-          const int sb = local & 1;
-          w = mbar_wait(&tfull[sb], (local >> 1) & 1, abort_flag);
+      int buf = local & 1;
+      if constexpr (SUMS) {
+        // this warp's chunks, four at most (SwiGLU: two of gate, two of up)
+        float sum[4][32] = {};
+        auto at = [&](int i) { return lanes + buf * BN_MAX + 32 * half + (wide ? 64 * (i & 1) + (i >> 1) * bn_out : 64 * i); };
+        const int mine = rows_in ? (nch - half + 1) / 2 : 0;
+        auto has = [&](int i) { return (wide ? i & 1 : i) < mine; };
+        for (int k0 = 0;; ++local) {
+          buf = local & 1;
+          w = mbar_wait(&tfull[buf], (local >> 1) & 1, abort_flag);
           if (!__all_sync(0xffffffffu, w)) {
             ok = false;
             break;
           }
           tc_fence_after();
-#pragma unroll 1
-          for (int c = half; c < nch && rows_in; c += 2)
-#pragma unroll 1
-            for (int at = 32 * c; at < bn; at += wide ? bn_out : bn) {  // SwiGLU: the chunk of gate, then of up
-              uint32_t acc[32], old[32];
-              tmem_ld32(lanes + sb * ACC + at, acc);
-              if (k0 > kstep) tmem_ld32(sum_tm + at, old);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (has(i)) {
+              uint32_t acc[32];
+              tmem_ld32(at(i), acc);
               tmem_ld_wait();
               tmem_reg_fence32(acc);
-              if (k0 > kstep) {
-                tmem_reg_fence32(old);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) acc[j] = __float_as_uint(__uint_as_float(acc[j]) + __uint_as_float(old[j]));
-              }
-              tmem_st32(sum_tm + at, acc);
+              for (int j = 0; j < 32; ++j) sum[i][j] += __uint_as_float(acc[j]);
             }
-          tmem_st_wait();
+          k0 += kstep;
+          if (k0 >= kblocks) break;
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(tempty0 + sb * 8);
+          if (lane == 0) mbar_arrive_cluster(tempty0 + buf * 8);
         }
         if (!ok) break;
-      }
-      // v += the sum's chunk at column `at`
-      auto add_sum = [&](float (&v)[32], int at) {
-        if constexpr (SUMS) {
-          uint32_t old[32];
-          tmem_ld32(sum_tm + at, old);
-          tmem_ld_wait();
-          tmem_reg_fence32(old);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(old[j]);
+        for (int i = 0; i < 4; ++i)
+          if (has(i)) tmem_st32(at(i), *reinterpret_cast<uint32_t(*)[32]>(sum[i]));
+        tmem_st_wait();
+      } else {
+        w = mbar_wait(&tfull[buf], (local >> 1) & 1, abort_flag);
+        if (!__all_sync(0xffffffffu, w)) {
+          ok = false;
+          break;
         }
-      };
-      const int buf = local & 1;
-      w = mbar_wait(&tfull[buf], (local >> 1) & 1, abort_flag);
-      if (!__all_sync(0xffffffffu, w)) {
-        ok = false;
-        break;
+        tc_fence_after();
       }
-      tc_fence_after();
-      const uint32_t trow = lanes + buf * ACC;
+      const uint32_t trow = lanes + buf * BN_MAX;
       for (int c = half; c < nch && rows_in; c += 2, b ^= 1) {
         const int col = n0 + 32 * c;
         uint8_t* sbuf = ebuf + b * SUB;
@@ -427,7 +431,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
         if (!ok) break;
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(acc[j]);
-        add_sum(v, 32 * c);
         if (wide) tmem_ld32(trow + bn_out + 32 * c, acc);
         if (bias) add_bias32(v, bias + col, args.N - col);
         if (wide) {
@@ -438,7 +441,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pk::THREADS, 1)
           tmem_reg_fence32(acc);
 #pragma unroll
           for (int j = 0; j < 32; ++j) u[j] = __uint_as_float(acc[j]);
-          add_sum(u, bn_out + 32 * c);
           if (bias) add_bias32(u, bias + args.N + col, args.N - col);
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] *= u[j];
@@ -550,9 +552,9 @@ namespace rk {
 constexpr int WARPS = 8, THREADS = 32 * WARPS;
 constexpr int UNROLL = 4;  // 32-k blocks whose loads are in flight per warp
 // Steps of the K loop after which a warp adds its accumulators, rounding to
-// nearest, to its sums in shared memory: 2048 of its K, 16384 of the whole (see
-// Long sums above; one sign, K = 2^20: 8.6e-4 of the product without it).
-constexpr int SUMS_STEPS = 2048 / (32 * UNROLL);
+// nearest, to its sums in shared memory: 512 of its K, 4096 of the whole, SwiGLU
+// half (see Sums in parts above).
+constexpr int sums_steps(bool wide) { return (wide ? 256 : 512) / (32 * UNROLL); }
 }  // namespace rk
 
 template <typename T>
@@ -676,7 +678,7 @@ __global__ void __launch_bounds__(rk::THREADS) linear16_rows_kernel(const __grid
         }
       }
     }
-    if (++steps == SUMS_STEPS) {
+    if (++steps == sums_steps(WIDE)) {
       steps = 0;
       put();
     }
@@ -736,10 +738,10 @@ int encode_operand(CUtensorMap* tm, const void* base, long long rows, int K, lon
 // Pair-tile width: the one whose waves over the SM pairs, times the tile's
 // time, finish first.  The 48 stand for what a K block costs at any width (1024
 // rows x 4608 x 3584: 256 wide, one wave, 25.4 us; 128 wide, two, 29.2 us).
-int pair_width(int M, int cols, bool wide, int most, int clusters) {
-  int best = most;
+int pair_width(int M, int cols, bool wide, int clusters) {
+  int best = pk::BN_MAX;
   double best_t = 1e300;
-  for (int bn = most; bn >= 64; bn -= wide ? 64 : 32) {
+  for (int bn = pk::BN_MAX; bn >= 64; bn -= wide ? 64 : 32) {
     const long long tiles = static_cast<long long>((M + 255) / 256) * ((cols + bn - 1) / bn);
     const double t = static_cast<double>((tiles + clusters - 1) / clusters) * (bn + 48);
     if (t < best_t * 0.97) {
@@ -772,8 +774,7 @@ template <typename T, typename O, bool SUMS>
 int launch_pair16(const Linear16Args& a, L16Dev& d, cudaStream_t stream, int num_sms) {
   const bool wide = a.act == QI_ACT_SWIGLU;
   const int clusters = num_sms / 2;
-  const int most = SUMS ? (wide ? pk::SUMS_BN_WIDE : pk::SUMS_BN) : pk::BN_MAX;
-  d.bn = pair_width(a.M, (wide ? 2 : 1) * a.N, wide, most, clusters);
+  d.bn = pair_width(a.M, (wide ? 2 : 1) * a.N, wide, clusters);
   const int bn_out = wide ? d.bn / 2 : d.bn;
   d.tiles_m = (a.M + pk::BM - 1) / pk::BM;
   d.tiles_n = (a.N + bn_out - 1) / bn_out;
@@ -793,6 +794,21 @@ int launch_pair16(const Linear16Args& a, L16Dev& d, cudaStream_t stream, int num
     return QI_ERR_CUDA;
   static unsigned long long attr_done = 0;
   const auto fn = linear16_pair_kernel<T, O, SUMS>;
+  if (SUMS) {
+    // The register split counts on LAUNCH_REGS per thread at launch: with fewer,
+    // the epilogue warps would wait for theirs without end.  A build that gave the
+    // kernel another number is refused
+    static int checked = 0;
+    if (!__atomic_load_n(&checked, __ATOMIC_ACQUIRE)) {
+      cudaFuncAttributes fa;
+      if (cudaFuncGetAttributes(&fa, reinterpret_cast<const void*>(fn)) != cudaSuccess) {
+        cudaGetLastError();
+        return QI_ERR_CUDA;
+      }
+      if (fa.numRegs != pk::LAUNCH_REGS) return QI_ERR_UNSUPPORTED;
+      __atomic_store_n(&checked, 1, __ATOMIC_RELEASE);
+    }
+  }
   if (smem_optin(reinterpret_cast<const void*>(fn), pk::SMEM_BYTES, &attr_done) != QI_OK) return QI_ERR_CUDA;
   const int tiles = d.tiles_m * d.tiles_n;
   return launch16(fn, 2u * (tiles < clusters ? tiles : clusters), pk::THREADS, pk::SMEM_BYTES, d, stream);
@@ -826,7 +842,7 @@ int launch_typed(const Linear16Args& a, cudaStream_t stream) {
   d.N = a.N;
   d.K = a.K;
   d.act = a.act;
-  if (a.K > pk::sums_min_k<O>()) return launch_pair16<T, O, true>(a, d, stream, device_num_sms());
+  if (a.K > pk::sums_min_k<T, O>(a.act == QI_ACT_SWIGLU)) return launch_pair16<T, O, true>(a, d, stream, device_num_sms());
   return launch_pair16<T, O, false>(a, d, stream, device_num_sms());
 }
 

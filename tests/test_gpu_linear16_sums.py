@@ -1,9 +1,9 @@
 """Accuracy of qi_linear_16bit's FP32 sums against 64 bits, for long K and in
 norm: sharper than the element bounds of a K-long sum, which grow with K.
 
-The tensor cores truncate: every product and every running sum of a part of
-the kernel's 2048 values of K loses at most one step of 2^-23 of that sum; the
-parts' sums (K / 2048 at most, and 8 warps') are rounded to nearest, again at
+The tensor cores truncate: every product and every running sum of one of the
+kernel's parts of 768 values of K at most loses at most one step of 2^-23 of that sum;
+the parts' sums (K / 512 at most, and 8 warps') are rounded to nearest, again at
 most 2^-23 each.
 """
 import pytest
@@ -27,14 +27,14 @@ def rand(shape, seed, dtype=F32, scale=1.0):
 def test_long_sums_of_one_sign(dtype, out_dtype, M, act):
     """A million products of one sign: a single truncated sum would lose 7e-3 of
     them (measured), so would its 16-bit result.  Per element, with T the sum
-    and h the half step of out: e = (2048 + K / 2048 + 16) 2^-23 T; silu of these
+    and h the half step of out: e = (768 + K / 512 + 16) 2^-23 T; silu of these
     sums (about 40) is the sum itself, plus 2^-19; SwiGLU multiplies two of them."""
     K, N = (1 << 20) + 8, 32
     wide = 2 if act == Q.ACT_SWIGLU else 1
     x, w = rand((M, K), 1, dtype, 2.0**-7).abs(), rand((wide * N, K), 2, dtype, 2.0**-7).abs()
     t = x.double() @ w.double().T
     assert 30 < float(t.min()) and float(t.max()) < 60
-    e = (2048 + K / 2048 + 16) * 2**-23 * t
+    e = (768 + K / 512 + 16) * 2**-23 * t
     want = t
     if act == Q.ACT_SWIGLU:
         s, u = t[:, :N] * torch.sigmoid(t[:, :N]), t[:, N:]
@@ -57,7 +57,7 @@ def test_first_lengths_in_parts(out_dtype, K, M, N):
     bias, gate, res = rand((N,), 5, dtype), rand((N,), 6), rand((M, N), 7, out_dtype)
     t = x.double().abs() @ w.double().abs().T + bias.double().abs()
     y = (x.double() @ w.double().T + bias.double()) * gate.double()
-    e = (2048 + K / 2048 + 17) * 2**-23 * t * gate.double().abs() + 2**-23 * y.abs()
+    e = (768 + K / 512 + 17) * 2**-23 * t * gate.double().abs() + 2**-23 * y.abs()
     want = y + res.double()
     e = e + 2**-23 * want.abs()
     tol = e + torch.finfo(out_dtype).eps / 2 * (want.abs() + e)
@@ -71,20 +71,20 @@ def test_first_lengths_in_parts(out_dtype, K, M, N):
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("M", [1, 3, 8, 9, 16, 17, 130, 600])
-@pytest.mark.parametrize("K", [64, 1000, 2048, 3584, 4096, 4104, 18944])
+@pytest.mark.parametrize("K", [64, 512, 520, 768, 776, 1000, 1032, 1544, 2048, 3584, 4096, 4104, 18944])
 def test_fp32_results_in_norm(dtype, M, K):
     """FP32 outputs of every kernel and epilogue in norm, with random signs.  Of n
     additions to one sum, which grows as the square root of their number, each
-    loses at most 2^-23 of it: 2/3 n 2^-23 of the result.  n = K / 16, parts of
-    2048 from K > 4096 on; with up to 16 rows eight warps share K.  A sum of few
+    loses at most 2^-23 of it: 2/3 n 2^-23 of the result.  n = K / 16, at most 48
+    (parts of 768, SwiGLU 24 of 384); with up to 16 rows eight warps share K.  A sum of few
     terms, of parts or of warps adds 2^-22.  The loss goes with the sums' size s,
     not with the result's: under a slope of 1.13 (silu, GELU) or times the other
     factor (SwiGLU) it is s times theirs; their own arithmetic adds 2^-18."""
     N = 328
     x, w, w2 = rand((M, K), 11, dtype), rand((N, K), 12, dtype, K**-0.5), rand((N, K), 13, dtype, K**-0.5)
     bias, gate, res = rand((N,), 14, dtype), rand((N,), 15), rand((M, N), 16)
-    tiles = (2048 if K > 4096 else K) / 16
-    n, n_wide = (K / 128 if M <= most else tiles for most in (16, 8))  # SwiGLU: up to 8 rows
+    n = min(48, K / 128 if M <= 16 else K / 16)
+    n_wide = min(24, K / 128 if M <= 8 else K / 16)
     b, b_wide = (2 / 3 * m * 2**-23 + 2**-22 for m in (n, n_wide))
     a, u = x.double() @ w.double().T, x.double() @ w2.double().T
 
