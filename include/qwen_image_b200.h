@@ -203,27 +203,34 @@ enum { QI_ACT_NONE = 0, QI_ACT_GELU = 1, QI_ACT_SILU = 2, QI_ACT_SWIGLU = 3 };
  * key rows [k_begin[b], k_end[b]) of k and v (device arrays of `batch` int32;
  * packed sequences pass an array of batch + 1 offsets as begin and the same
  * array from its second entry as end; a cache with a slot per sequence passes
- * each slot's start and fill).  The query ranges must not overlap.  With Lq
- * queries and Lk keys, causal != 0 lets query i see the keys j <= i + Lk - Lq:
- * the queries are the sequence's last Lq positions, so Lq = 1 is one new token
- * against a cache.  A query that sees no key gives zeros.  Rows of out in no
- * query range are not written.  What rows of k and v outside a sequence's
- * range hold, or at positions a query does not see, does not reach that
- * query's result, NaN and infinities included.  out may be q itself (same
- * pointer and strides); otherwise it shares no element with q, k or v
- * (QI_ERR_ARG).
+ * each slot's start and fill).  The query ranges must not overlap; key ranges
+ * may.  With Lq queries and Lk keys, causal != 0 lets query i see the keys
+ * j <= i + Lk - Lq: the queries are the sequence's last Lq positions, so Lq = 1
+ * is one new token against a cache.  A query that sees no key, or only scores
+ * of minus infinity, gives zeros.  Rows of out in no query range are not
+ * written.  What rows of k and v outside a sequence's range hold, or at
+ * positions a query does not see, does not reach that query's result, NaN and
+ * infinities included.
+ * out may be q itself (same pointer and strides); otherwise its memory lies
+ * apart from that of q, k and v (QI_ERR_ARG): byte ranges that do not meet, or,
+ * in rows of one buffer (same row stride), heads that lie apart in each row.
  * Element (row, head, d) of x is x[row * x_row + head * x_head + d]; strides
  * are in elements, positive and multiples of 8, pointers 16-byte aligned
- * (QI_ERR_ALIGN); rows and heads of out must not overlap one another.  total_q and
- * total_k are the rows of q / out and of k / v; ranges are clipped to them.
+ * (QI_ERR_ALIGN); rows and heads of out must not overlap one another.  total_q
+ * and total_k are the rows of q / out and of k / v; ranges are clipped to them.
  * dtype is QI_DT_BF16 or QI_DT_F16 (all four tensors); |scale| < 2e38
- * (QI_ERR_ARG).  head_dim is a multiple
- * of 8, at most 128 (QI_ERR_UNSUPPORTED).  max_k >= the longest key range is a
- * hint that decides how keys are split over the device: a wrong one costs
- * time, not correctness.  workspace: at least
- * qi_prompt_attention_workspace(...) bytes, 16-byte aligned, not used by any
- * other call until this one has finished (QI_ERR_ARG when smaller; that size
- * is 0 and workspace may be NULL when the keys are not split).
+ * (QI_ERR_ARG), 0 and subnormal numbers included.  head_dim is a multiple of 8,
+ * at most 128 (QI_ERR_UNSUPPORTED).  max_k >= the longest key range is a hint
+ * that decides how keys are split over the device: a wrong one costs time, not
+ * correctness.  workspace: at least qi_prompt_attention_workspace(...) bytes,
+ * 16-byte aligned, not used by any other call until this one has finished
+ * (QI_ERR_ARG when smaller; that size is 0 and workspace may be NULL when the
+ * keys are not split).
+ * Scores (up to 2^127 in size), the softmax's maximum and sum and the sum over
+ * v are FP32; the weights are rounded to dtype before they meet v, the result
+ * once.  The tensor cores truncate the sum over v every 16 keys: off by up to
+ * 6e-9 of sum_j p_j |v_j| per key of one split (1.4e-3 at 262144 keys that are
+ * not split and v of one sign; 1e-5 at 4096).
  * Replaces attention_forward (cuda_kernels.cu:1162-1240) as the text encoder
  * uses it; exact counterpart of qi_sage_attention for causal = 0.            */
 int qi_prompt_attention(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
@@ -241,15 +248,17 @@ long long qi_prompt_attention_workspace(int heads, int kv_heads, int head_dim, i
  *   out[m, n] = residual[m, n] + gate[n] * act(sum_k x[m, k] w[n, k] + bias[n])
  * x [M, K] and w [N, K] are dtype (QI_DT_BF16 or QI_DT_F16) with leading
  * dimensions ldx and ldw, out [M, N] is out_dtype (dtype, or QI_DT_F32) with
- * ldo, sums are FP32 and rounded once into out.  bias (dtype), gate (FP32) and
- * residual (out_dtype, leading dimension ldr) may be NULL: 0, 1 and 0.
+ * ldo, sums are FP32 and rounded once into out (FP32 out: off by 8e-7 in norm
+ * at most for random signs, by 1e-6 (BF16) or 3e-6 (FP16) where all products
+ * have one sign).  bias (dtype), gate (FP32) and residual (out_dtype, leading
+ * dimension ldr) may be NULL: 0, 1 and 0.
  * act: QI_ACT_NONE, QI_ACT_GELU (tanh form), QI_ACT_SILU, or QI_ACT_SWIGLU,
  * where w holds 2N rows and bias 2N values and
  *   act(...) = silu(x . w[n] + bias[n]) * (x . w[N + n] + bias[N + n]).
  * residual may be out itself (same pointer and leading dimension); otherwise
- * out overlaps no input (QI_ERR_ARG).  Any M >= 0, N and K >= 1; all pointers
- * 16-byte aligned and all leading dimensions multiples of 16 bytes
- * (QI_ERR_ALIGN).
+ * the bytes from out's first to its last element meet none of an input's
+ * (QI_ERR_ARG).  Any M >= 0, N and K >= 1; all pointers 16-byte aligned and all
+ * leading dimensions multiples of 16 bytes (QI_ERR_ALIGN).
  * Replaces the cuBLAS BF16 products with separate bias, activation and
  * residual kernels behind them (cuda_kernels.cu:4535-4596).                 */
 int qi_linear_16bit(const void* x, long long ldx, int M, int K, const void* w, long long ldw, int N, int dtype,

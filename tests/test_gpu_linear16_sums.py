@@ -106,3 +106,30 @@ def test_fp32_results_in_norm(dtype, M, K):
     s = a.square().mean().sqrt()
     close(Q.linear_16bit(x, torch.cat([w, w2]), act=Q.ACT_SWIGLU, out_dtype=F32), silu * u,
           b_wide * s * (1.13 * u.norm() + silu.norm()) + 2**-18 * (silu * u).norm())
+
+
+def test_parts_are_added_up_the_same_every_time():
+    """FP32 sums in parts: eager on two streams at once, and captured and replayed
+    on other inputs."""
+    cases = [(rand((M, K), 20 + M, BF), rand((648, K), 21 + M, BF, K**-0.5)) for M, K in ((5, 9000), (40, 3584), (300, 3584), (2600, 1544))]
+    acts = (Q.ACT_NONE, Q.ACT_SWIGLU)
+    run = lambda: [Q.linear_16bit(x, w, act=a, out_dtype=F32) for x, w in cases for a in acts]  # noqa: E731
+    first = run()
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(run())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for o in outs for a, b in zip(o, first))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run()
+    for x, _ in cases:
+        x.copy_(x.flip(0) * 0.5)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(captured, run()))
+    Q.prompt_ops_check()
