@@ -230,7 +230,7 @@ enum { QI_ACT_NONE = 0, QI_ACT_GELU = 1, QI_ACT_SILU = 2, QI_ACT_SWIGLU = 3 };
  * v are FP32; the weights are rounded to dtype before they meet v, the result
  * once.  The tensor cores truncate the sum over v every 16 keys: off by up to
  * 6e-9 of sum_j p_j |v_j| per key of one split (1.4e-3 at 262144 keys that are
- * not split and v of one sign; 1e-5 at 4096).
+ * not split and v of one sign; 3e-5 at 4096).
  * Replaces attention_forward (cuda_kernels.cu:1162-1240) as the text encoder
  * uses it; exact counterpart of qi_sage_attention for causal = 0.            */
 int qi_prompt_attention(const void* q, long long q_row, long long q_head, const void* k, long long k_row,

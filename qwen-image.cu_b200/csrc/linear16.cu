@@ -7,9 +7,10 @@
 // Two kernels, chosen by the number of rows M of x:
 //   * pair kernel: tcgen05 on CTA pairs, 256 x bn output tiles, persistent, the
 //     epilogue of one tile under the main loop of the next.  Bound by the tensor
-//     cores: 8192 x 12288 x 3584 with GELU 475-490 us (1470-1520 TFLOP/s, tensor
-//     cores busy for 97% of the time).  With one wave of narrow tiles by the
-//     copies of x and w, about 0.25 us per 64 of K.
+//     cores: 8192 x 12288 x 3584 with GELU 474-496 us (1460-1520 TFLOP/s, tensor
+//     cores busy for 97% of the time), back to back under the power cap 575-591.
+//     With one wave of narrow tiles by the copies of x and w, about 0.25 us per 64
+//     of K.
 //   * rows kernel (up to 16 rows): w streamed through warp-level MMAs.  Bound by
 //     the bytes of w.
 #include "qi_internal.h"
@@ -118,7 +119,8 @@ constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS);
 // sums in parts: registers per thread at launch, then of the first warpgroup and
 // of the epilogue's two
 constexpr int LAUNCH_REGS = 168, PRODUCER_REGS = 88, EPI_REGS = 208;
-static_assert(32 * (EPI_WARP0 * PRODUCER_REGS + EPI_WARPS * EPI_REGS) <= THREADS * LAUNCH_REGS, "register split exceeds the launch");
+static_assert(32 * (EPI_WARP0 * PRODUCER_REGS + EPI_WARPS * EPI_REGS) <= THREADS * LAUNCH_REGS,
+              "register split exceeds the launch");
 // Sums in parts.  The tensor cores truncate every addition to an accumulator, so
 // its error grows with K: 9e-10 K (BF16) or 1.3e-9 K (FP16) of the product in norm,
 // with one sign 1.6e-9 or 5e-9 K at small K, 6.7e-9 K (FP16) at large.  Where that
@@ -783,9 +785,9 @@ int launch_pair16(const Linear16Args& a, L16Dev& d, cudaStream_t stream, int num
   d.tiles_n = (a.N + bn_out - 1) / bn_out;
   if (static_cast<long long>(d.tiles_m) * d.tiles_n > 0x3fffffff) return QI_ERR_UNSUPPORTED;
   // Two K blocks per stage for narrow tiles, where a stage's waits and barriers
-  // cost more than one block of MMAs (N 4608, K 3584, one / two: 96 rows 17.9 /
-  // 16.0 us, 512 rows 19.4 / 17.9); wider tiles need the stages (700 rows x 3584
-  // x 14336, 160 wide: 62 / 66 us)
+  // cost more than one block of MMAs (N 4608, K 3584, one / two: 96 rows 17.5 /
+  // 15.7 us, 512 rows 18.9 / 17.6); wider tiles gain nothing (700 rows x 3584 x
+  // 14336, 160 wide: 69.1 / 69.3 us)
   d.atoms = d.bn <= 128 ? 2 : 1;
   d.stages = pk::stage_room<O>() / (d.atoms * (pk::A_BLOCK + d.bn / 2 * BK * 2));
   if (d.stages > pk::MAX_STAGES) d.stages = pk::MAX_STAGES;
@@ -822,7 +824,8 @@ int launch_rows(const Linear16Args& a, cudaStream_t stream) {
   constexpr int COLS = WIDE ? 16 : 16 * R;
   constexpr int smem = rk::WARPS * 8 * G * (16 * R + 4) * 4;
   static_assert(smem <= 48 * 1024, "shared memory that needs no opt-in");
-  return launch16(linear16_rows_kernel<T, O, G, R, WIDE>, static_cast<unsigned>((a.N + COLS - 1) / COLS), rk::THREADS, smem, a, stream);
+  return launch16(linear16_rows_kernel<T, O, G, R, WIDE>, static_cast<unsigned>((a.N + COLS - 1) / COLS), rk::THREADS, smem, a,
+                  stream);
 }
 
 template <typename T, typename O>

@@ -22,13 +22,22 @@
 // S and O fill TMEM, so a tile's next S waits for its P V, and the other tile's
 // products run under its softmax.
 //
-// Measured (device time, calls in one graph): 8192 causal tokens, 28 heads on 4
-// of 128: 420-450 us, 1070-1150 TFLOP/s, tensor cores busy for 55% of the time;
-// 24 heads x 2 x 4352 keys: 435 us.  Bound by the chain S -> softmax -> P V of
-// each tile, not by the exponentials (polynomials for a part of them were
-// slower).  One token each against 16 caches of up to 4096: 23.4 us, one cache of
-// 30000: 23.3 us, of which reading K and V takes 9: the rest is set-up, the
-// first loads' latency and the joining launch.
+// Measured (device time of calls in one graph; back to back, where the power cap
+// sets the clock, in brackets): 8192 causal tokens, 28 heads on 4 of 128: 431-434 us
+// (500), 1110 TFLOP/s, tensor cores busy for 53% of the time; 24 heads x 2 x 4352
+// keys: 428-473 us (495).  A key block of two tiles takes some 4000 clocks, of which
+// its products and its exponentials each need 2048 and overlap: bound by the chain S
+// -> softmax -> P V of each tile, a thread per row with two warps per scheduler to
+// hide its latencies.  (The two-tile kernels spill a few registers: 68 bytes stored
+// and 144 loaded per thread at heads of 128, 28 and 100 at 64.)  One token each
+// against 16 caches of up to 4096: 24.2-25.9 us, one cache of 30000: 24.1-25.5 us, of
+// which reading K and V takes 9: the rest is set-up, the first loads' latency and
+// the joining launch.
+//
+// Sums.  The tensor cores truncate O every 16 keys.  Off by up to 6e-9 of sum p |v|
+// per key of a split: 3e-5 at 4096 keys with v of one sign, 1.4e-3 at 262144 that are
+// not split (a half step of FP16 is 4.9e-4, of BF16 3.9e-3).  TMEM is full with two
+// tiles of heads of 128, so there is no room for a second sum.
 //
 // V guard.  A masked weight is 0, but 0 times a NaN or infinity of v is NaN: in
 // blocks with masked keys (the last ones) the guard clears the V rows that no
